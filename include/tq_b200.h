@@ -52,6 +52,9 @@ typedef struct CUstream_st* tq_stream_t; /* same type as cudaStream_t */
 #define TQ_STATUS_BAD_BLOCK 1 /* a block-table entry was outside [0, num_blocks) and was clamped */
 #define TQ_STATUS_TIMEOUT 2   /* a bounded wait on an async copy ran out */
 #define TQ_STATUS_BAD_SLOT 4  /* a slot index was >= num_blocks * block_size and was skipped */
+#define TQ_STATUS_BAD_POSITION 8 /* a position was outside the rotary table and was clamped */
+#define TQ_STATUS_NO_BLOCKS 16   /* a request got no slots: the free blocks were used up */
+#define TQ_STATUS_TOO_LONG 32    /* a request's rows, blocks or queries exceed what the call's tensors hold; it was cut or left out */
 
 /* Library version, (major << 16) | minor.  Host only. */
 int tq_version(void);
@@ -237,6 +240,99 @@ int tq_packed_attention(const void* Q, const void* Q_proj, const uint8_t* k_idx,
                         const void* k_rnorm, const void* k_norm, const uint8_t* v_idx, const void* v_norm,
                         const float* centroids, float corr_scale, int BH, int Sk, int bits, int num_splits,
                         void* workspace, int64_t workspace_bytes, void* out, tq_stream_t stream);
+
+/* Rotary positions of query and key heads, out of place or in place (q_out = q,
+ * k_out = k; other overlaps are not allowed).  q, q_out: [rows, num_q_heads,
+ * head_dim], k, k_out: [rows, num_kv_heads, head_dim] of dtype; strides: 8
+ * element strides, (row, head) of q, k, q_out, k_out.  Values 0 .. rotary_dim
+ * of each head are turned, the rest copied: pairs (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) when interleaved; inverse turns back (the gradient of the turn).
+ * table: fp32 [table_rows, rotary_dim], cosines then sines of the
+ * rotary_dim / 2 angles of a position; positions: int64 (wide_positions) or
+ * int32 [rows], clamped to the table with TQ_STATUS_BAD_POSITION.  Interleaved
+ * pairs start on their own size. */
+int tq_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, const int64_t* strides,
+              const void* positions, int wide_positions, const float* table, int64_t table_rows, int64_t rows,
+              int num_q_heads, int num_kv_heads, int head_dim, int rotary_dim, int interleaved, int inverse,
+              int32_t* status, tq_stream_t stream);
+
+/* Bytes of one 16-token page of the 8-bit cache: e4m3 codes of K [16][head_dim],
+ * of V [16][head_dim], the fp32 scales of K and V, 24 unused bytes; negative
+ * for a head_dim other than 64 and 128.  The cache is uint8 [num_blocks,
+ * num_kv_heads, block_size / 16 * page_bytes], as the packed one.  Host only. */
+int tq_cache8_page_bytes(int head_dim);
+
+/* New K/V rows into the 8-bit cache.  A scale is 2^e with the smallest e >= -100
+ * for which no finite value of the page's rows is above 448 * 2^e; a code is
+ * the e4m3 value nearest to x / scale (ties to even; infinities saturate, a NaN
+ * stays one).  A page whose first slot is among the rows is begun anew: its
+ * scale comes from these rows alone.  Otherwise the page keeps the larger of
+ * its scale and theirs, and the codes before them are rescaled when it grows
+ * (exact, but for codes that become subnormal).  Codes behind the last row
+ * written are left as they were.
+ *
+ * key, value: as in tq_compress_paged, with head_dim 64 or 128; rows, heads
+ * and the cache start on 16 bytes.  slot_mapping: int64 [n_tokens]; negative
+ * slots are skipped, slots beyond the cache are skipped and flagged.  Rows of
+ * one page stand next to one another in ascending order, as sequences bring
+ * them; if a call names a page in two places, or a slot twice, that page's
+ * content is not specified. */
+int tq_quantize8_paged(const void* key, const void* value, int in_dtype, int64_t k_stride_token, int64_t k_stride_head,
+                       int64_t v_stride_token, int64_t v_stride_head, void* cache, int64_t num_blocks, int block_size,
+                       const int64_t* slot_mapping, int64_t n_tokens, int n_kv_heads, int head_dim, int32_t* status,
+                       tq_stream_t stream);
+
+/* Bytes of workspace tq_attend8_paged needs.  Host only. */
+int64_t tq_attend8_workspace_bytes(int64_t num_rows, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                                   int max_queries, int max_pages_per_seq);
+
+/* Attention over the 8-bit cache, causal at the end of each sequence.  out, q:
+ * [num_rows, num_q_heads, head_dim] of io_dtype (fp16 or bf16), 16-byte aligned.
+ * Rows query_start_loc[i] .. query_start_loc[i + 1] (int32 [num_seqs + 1],
+ * ascending) are the last tokens of sequence i, whose seq_lens[i] tokens, these
+ * included, are in the cache; query_start_loc = NULL: row i is sequence i's
+ * only one.  Row j of n sees the first seq_lens[i] - n + j + 1 tokens; one that
+ * sees none becomes zeros.  max_queries: at least the most rows of a sequence
+ * (the ones beyond are left out and flagged).  Rows behind the last sequence
+ * are left as they were, or become zeros when zero_tail.  block_tables,
+ * bt_stride, seq_lens, max_pages_per_seq, workspace, status: as in
+ * tq_decode_paged. */
+int tq_attend8_paged(void* out, const void* q, int io_dtype, const void* cache, int64_t num_blocks, int block_size,
+                     const int32_t* block_tables, int64_t bt_stride, const int32_t* seq_lens, const int32_t* query_start_loc,
+                     float sm_scale, void* workspace, int64_t workspace_bytes, int32_t* status, int64_t num_rows,
+                     int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int max_queries,
+                     int max_pages_per_seq, int zero_tail, tq_stream_t stream);
+
+/* Step tables from the requests' lengths.  Request i has context_lens[i] tokens
+ * in the cache, in the first ceil(context / block_size) blocks of row i of
+ * block_tables, and brings query_lens[i] new ones (negative counts as 0).  The
+ * blocks it lacks come from the top of the stack free_blocks[0 ..
+ * *free_count) in the order of the requests and are written into its row of
+ * block_tables.  Out: slot_mapping and positions (int64 [num_rows]) of the new
+ * tokens, request after request; seq_lens[i] = context + query;
+ * query_start_loc (int32 [num_requests + 1]); *new_free_count, the height of the
+ * stack afterwards.  free_blocks and *free_count are not changed, so that a
+ * repeated call gives the same tables.  Rows behind the last request get slot
+ * -1 and position 0.  A request for which the blocks do not suffice
+ * (TQ_STATUS_NO_BLOCKS), or whose rows or blocks do not fit num_rows or
+ * table_width (TQ_STATUS_TOO_LONG), takes none: its rows get slot -1, its
+ * seq_lens entry stays the context.  No output may overlap an input. */
+int tq_plan_step(const int32_t* query_lens, const int32_t* context_lens, int32_t* block_tables, int64_t bt_stride,
+                 const int32_t* free_blocks, const int32_t* free_count, int64_t* slot_mapping, int64_t* positions,
+                 int32_t* seq_lens, int32_t* query_start_loc, int32_t* new_free_count, int32_t* status,
+                 int64_t num_requests, int64_t table_width, int64_t num_free, int block_size, int64_t num_rows,
+                 tq_stream_t stream);
+
+/* The blocks of the requests with ended[i] != 0 (the first ceil(context /
+ * block_size) of their rows) go onto the stack, request after request:
+ * free_blocks[*free_count ..); *new_free_count is its new height and
+ * new_context_lens[i] 0 for them, context_lens[i] for the others.  *free_count
+ * is not changed.  What exceeds the stack's num_free places is dropped and
+ * flagged (TQ_STATUS_TOO_LONG). */
+int tq_release_blocks(const uint8_t* ended, const int32_t* context_lens, const int32_t* block_tables, int64_t bt_stride,
+                      int32_t* free_blocks, const int32_t* free_count, int32_t* new_context_lens, int32_t* new_free_count,
+                      int32_t* status, int64_t num_requests, int64_t table_width, int64_t num_free, int block_size,
+                      tq_stream_t stream);
 
 #ifdef __cplusplus
 }

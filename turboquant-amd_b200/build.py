@@ -21,7 +21,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "turboquant", "lib", "libtq_b200.so")
 HOST_LIB = os.path.join(HERE, "turboquant", "lib", "_tq_host.so")
-SOURCES = ["tq_compress.cu", "tq_decode.cu", "tq_packed_attention.cu"]
+SOURCES = ["tq_compress.cu", "tq_decode.cu", "tq_packed_attention.cu", "tq_rotary.cu", "tq_cache8.cu", "tq_attend8.cu",
+           "tq_plan.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
          "-Xcompiler", "-fPIC", "-Xptxas", "-v"]

@@ -1,0 +1,557 @@
+// Attention over the 8-bit paged cache (tq_cache8.cuh): queries of one token per sequence, of a few, or of a chunk of a prompt whose
+// keys are in the cache already.
+//
+// For a query row (token j of n in a sequence of `len` tokens, head h) with KV head h / G:
+//   s_k = sm_scale * <q, K_k> * kscale(page of k)      for k < len - n + j + 1
+//   out = sum_k 2^(s_k - m) vscale(page of k) V_k / sum_k 2^(s_k - m)      (s in units of log2)
+//
+// Bound: HBM, the 2 D + 2 bytes of a cached token and head, at about D / 16 products and 70 other instructions a page and warp.
+#include "tq_cache8.cuh"
+
+namespace tq {
+namespace {
+
+struct Attend8Params {
+    void* out;
+    const void* q;
+    const uint8_t* cache;
+    const int32_t* tables;
+    const int32_t* seq_lens;
+    const int32_t* starts;          // [seqs + 1], null: row i is sequence i's only one
+    float* partials;
+    int32_t* status;
+    int64_t num_blocks, table_stride;
+    float scale_log2;
+    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, tile_rows, chunk_pages, chunks, merge_blocks, zero_tail;
+};
+
+constexpr float kNothing = -3e38f;      // reference of a row that has seen no token: below every score, and finite, so that differences are numbers
+constexpr float kLazy = 8.f;            // a score may pass the reference by so much before it is raised
+constexpr float kHeadroom = 6.f;        // weights are multiplied by 2^6: at most 2^14 in fp16, full precision down to 2^-20 of the largest
+
+// What one warp holds while it walks over pages of a sequence, for 8 * NT query rows against one KV head.
+//
+// Scores: m16n8k16 products with 16 tokens as M and query rows as N.  A lane (g = lane / 4, t = lane % 4) reads 16-byte pieces t (and t + 4) of
+// tokens g and g + 8: four dims are one operand register pair, with the query laid out alike, so the codes need no shuffling at all.
+// Values: V^T as the A operand (dims as M).  A lane reads dims D/8 * g .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9 - whole 128-byte
+// rows - and a byte permute pairs the tokens.  Weights go from accumulator to operand layout by two movmatrix.
+template <int D, int NT>
+struct Rows {
+    static constexpr int kSteps = D / 16;      // products of a page's scores, and m-tiles of its values
+    uint32_t q[NT][kSteps][2];
+    float scale[NT][2];                        // of the two columns of this lane
+    float m[NT][2], u[NT][2], l[NT][2];        // references of weights and of weights * vscale, denominators of this lane
+    float o[kSteps][NT][4];
+    int limit[NT][2];                          // tokens that the column sees
+    int min_limit, max_limit;
+};
+
+template <int D>
+struct Page {
+    uint4 k[2][D / 64];
+    uint32_t v[4][D / 32];
+    float2 scales;
+};
+
+template <int D>
+__device__ __forceinline__ const uint8_t* page_address(const Attend8Params& p, int page, int block, int kvh) {
+    return p.cache + ((static_cast<int64_t>(block) * p.kv_heads + kvh) * p.pages_per_block + page % p.pages_per_block) *
+                         static_cast<int64_t>(cache8_page_bytes(D));
+}
+
+template <int D>
+__device__ __forceinline__ void load_keys(Page<D>& x, const uint8_t* base, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) x.k[r][c] = __ldg(reinterpret_cast<const uint4*>(base + (g + 8 * r) * D + 64 * c + 16 * t));
+    x.scales = __ldg(reinterpret_cast<const float2*>(base + cache8_scale_off(D)));
+}
+
+template <int D>
+__device__ __forceinline__ void load_values(Page<D>& x, const uint8_t* base, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint8_t* at = base + kPageTokens * D + (2 * t + (i & 1) + 8 * (i >> 1)) * D + D / 8 * g;
+        if constexpr (D == 128) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(at));
+            x.v[i][0] = w.x; x.v[i][1] = w.y; x.v[i][2] = w.z; x.v[i][3] = w.w;
+        } else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(at));
+            x.v[i][0] = w.x; x.v[i][1] = w.y;
+        }
+    }
+}
+
+// Query rows r0 .. r0 + 8 NT of a sequence as B operands.  fp16 queries are used as they are; bf16 ones are brought into the range of
+// fp16 by a power of two for each row, which costs no bit of values within 2^-14 of the row's largest.
+template <int D, int NT, bool BF16>
+__device__ __forceinline__ void load_queries(Rows<D, NT>& w, const Attend8Params& p, int first_row, int kvh, int r0, int nrows, int len, int nq, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = r0 + 8 * n + g;
+        uint32_t x[D / 64][8];
+        if (r < nrows) {
+            const int token = r / p.group, head = kvh * p.group + r - token * p.group;
+            const uint16_t* src = static_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(first_row + token) * p.q_heads + head) * D + 16 * t;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(src + 64 * c)), b = __ldg(reinterpret_cast<const uint4*>(src + 64 * c + 8));
+                x[c][0] = a.x; x[c][1] = a.y; x[c][2] = a.z; x[c][3] = a.w;
+                x[c][4] = b.x; x[c][5] = b.y; x[c][6] = b.z; x[c][7] = b.w;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[c][i] = 0;
+        }
+        float row_scale = p.scale_log2;
+        if constexpr (BF16) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = max(most, max(x[c][i] & 0x7fffu, x[c][i] >> 16 & 0x7fffu));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int e = min(max(static_cast<int>(most >> 7) - 127, -120), 120);
+            const float down = exp2_int(-e);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[c][i] = pack_half2(__uint_as_float(x[c][i] << 16) * down, __uint_as_float(x[c][i] & 0xffff0000u) * down);
+            row_scale *= exp2_int(e);
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w.q[n][4 * c + i][0] = x[c][2 * i];
+                w.q[n][4 * c + i][1] = x[c][2 * i + 1];
+            }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            w.scale[n][j] = __shfl_sync(0xffffffffu, row_scale, (2 * t + j) * 4);
+            const int row = r0 + 8 * n + 2 * t + j;
+            w.limit[n][j] = len - nq + min(row, nrows - 1) / p.group + 1;
+            w.m[n][j] = w.u[n][j] = kNothing;
+            w.l[n][j] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < Rows<D, NT>::kSteps; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.o[i][n][j] = 0.f;
+    w.min_limit = len - nq + r0 / p.group + 1;
+    w.max_limit = len - nq + min(r0 + 8 * NT - 1, nrows - 1) / p.group + 1;
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void page_scores(float (&s)[NT][4], const Rows<D, NT>& w, const Page<D>& x) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+        const uint32_t a[4] = {x.k[0][c].x, x.k[0][c].y, x.k[0][c].z, x.k[0][c].w}, b[4] = {x.k[1][c].x, x.k[1][c].y, x.k[1][c].z, x.k[1][c].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a0 = e4m3x2_to_half2(a[i] & 0xffffu), a1 = e4m3x2_to_half2(b[i] & 0xffffu);
+            const uint32_t a2 = e4m3x2_to_half2(a[i] >> 16), a3 = e4m3x2_to_half2(b[i] >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], a0, a1, a2, a3, w.q[n][4 * c + i][0], w.q[n][4 * c + i][1]);
+        }
+    }
+}
+
+// Adds weights * V.  Tokens of the page from `visible` on count as zeros, whatever their codes say.
+template <int D, int NT, bool CUT>
+__device__ __forceinline__ void page_values(float (&o)[D / 16][NT][4], const Page<D>& x, const uint32_t (&weights)[NT][2], int visible, int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = !CUT || 2 * t + (j & 1) + 8 * (j >> 1) < visible ? x.v[j][i] : 0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = prmt(v[0], v[1], h ? 0x7362 : 0x5140), hi = prmt(v[2], v[3], h ? 0x7362 : 0x5140);
+            const uint32_t a0 = e4m3x2_to_half2(lo & 0xffffu), a1 = e4m3x2_to_half2(lo >> 16);
+            const uint32_t a2 = e4m3x2_to_half2(hi & 0xffffu), a3 = e4m3x2_to_half2(hi >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(o[2 * i + h][n], a0, a1, a2, a3, weights[n][0], weights[n][1]);
+        }
+    }
+}
+
+template <int D>
+__device__ __forceinline__ bool has_nan(const Page<D>& x, int from, int lane) {
+    const int t = lane & 3;
+    uint32_t found = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const uint32_t full = (x.v[j][i] & 0x7f7f7f7fu) + 0x01010101u;      // bit 7 of a byte: it is 0x7f
+            if (2 * t + (j & 1) + 8 * (j >> 1) >= from) found |= full & 0x80808080u;
+        }
+    return __any_sync(0xffffffffu, found != 0);
+}
+
+// One page.  The softmax keeps two references per column: m for the denominators and u, which includes the value scale 2^ev of the page, for the
+// products, whose fp16 weights then use their range whatever the pages' scales are.  Both are raised only where a score passes
+// them by 2^8: most pages need one vote and no shuffles.
+template <int D, int NT>
+__device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], float2 scales, int page, uint32_t (&weights)[NT][2]) {
+    const int g = (threadIdx.x & 31) >> 2;
+    const float ev = static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127);
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] *= w.scale[n][j & 1] * scales.x;
+    if (page * kPageTokens + kPageTokens > w.min_limit) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (page * kPageTokens + g + 8 * (j >> 1) >= w.limit[n][j & 1]) s[n][j] = -__uint_as_float(0x7f800000u);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) over |= fmaxf(s[n][j], s[n][j + 2]) > fminf(w.m[n][j], w.u[n][j] - ev) + kLazy;
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float most = fmaxf(s[n][j], s[n][j + 2]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float m = fmaxf(w.m[n][j], most), u = fmaxf(w.u[n][j], most + ev);
+                w.l[n][j] *= ex2(w.m[n][j] - m);
+                const float down = ex2(w.u[n][j] - u);
+#pragma unroll
+                for (int i = 0; i < Rows<D, NT>::kSteps; ++i) {
+                    w.o[i][n][j] *= down;
+                    w.o[i][n][j + 2] *= down;
+                }
+                w.m[n][j] = m;
+                w.u[n][j] = u;
+            }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w.l[n][j & 1] += ex2(s[n][j] - w.m[n][j & 1]);
+            e[j] = ex2(s[n][j] - (w.u[n][j & 1] - ev - kHeadroom));
+        }
+        weights[n][0] = movmatrix_trans(pack_half2(e[0], e[1]));      // tokens 2t, 2t + 1 of column g
+        weights[n][1] = movmatrix_trans(pack_half2(e[2], e[3]));
+    }
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void page_products(Rows<D, NT>& w, const Page<D>& x, const uint32_t (&weights)[NT][2], int page, int lane) {
+    const int first = page * kPageTokens;
+    if (first + kPageTokens <= w.min_limit) {
+        page_values<D, NT, false>(w.o, x, weights, kPageTokens, lane);
+        return;
+    }
+    const int most = min(w.max_limit - first, kPageTokens), least = max(min(w.min_limit - first, kPageTokens), 0);
+    if (most == least || !has_nan<D>(x, least, lane)) {
+        page_values<D, NT, true>(w.o, x, weights, most, lane);
+        return;
+    }
+    // A NaN that some columns see and others do not: 0 * NaN would reach the latter.  It counts as zero in the product, and a second
+    // one, of ones where NaN stand with ones where a column sees a token, says where it belongs.
+    const int g = lane >> 2, t = lane & 3;
+    Page<D> clean, marks;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const uint32_t nan = ((x.v[j][i] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u;
+            clean.v[j][i] = x.v[j][i] & ~(nan * 0xffu);
+            marks.v[j][i] = nan * 0x38u;               // 1.0 in e4m3
+        }
+    page_values<D, NT, true>(w.o, clean, weights, most, lane);
+    uint32_t sees[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        // the limit of column g of this tile is held by the lanes whose t is g / 2
+        const int lo = __shfl_sync(0xffffffffu, w.limit[n][0], g >> 1), hi = __shfl_sync(0xffffffffu, w.limit[n][1], g >> 1);
+        const int mine = (g & 1 ? hi : lo) - first;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            sees[n][h] = (2 * t + 8 * h < mine ? 0x3c00u : 0u) | (2 * t + 1 + 8 * h < mine ? 0x3c000000u : 0u);
+    }
+    float found[D / 16][NT][4] = {};
+    page_values<D, NT, true>(found, marks, sees, most, lane);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (found[i][n][j] > 0.f) w.o[i][n][j] = __uint_as_float(0x7fffffffu);
+}
+
+__device__ __forceinline__ void store_out(void* out, int64_t at, float x, bool bf16) {
+    if (bf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(out)[at] = __float2half_rn(x);
+}
+
+constexpr int kWarps = 4;
+
+// The rows of a sequence, inside the tensors whatever `starts` says; true when it has more than the launch is sized for, which are left out.
+__device__ __forceinline__ bool rows_of(const Attend8Params& p, int seq, int& first_row, int& nq) {
+    first_row = seq;
+    nq = 1;
+    if (!p.starts) return false;
+    first_row = min(max(p.starts[seq], 0), p.rows);
+    const int n = max(min(p.starts[seq + 1], p.rows) - first_row, 0);
+    nq = min(n, p.max_queries);
+    return n > p.max_queries;
+}
+
+// CTA: one chunk of pages of (sequence, KV head, tile of 8 NT query rows); its warps take a quarter of the pages each.
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32) attend8_kernel(const Attend8Params p) {
+    __shared__ float part_o[kWarps][8 * NT][D];
+    __shared__ float part_m[kWarps][8 * NT], part_l[kWarps][8 * NT];
+    pdl_wait();
+    pdl_release_if_small();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    // chunks of one item side by side, then the tiles of a KV head, which read the same pages
+    int rest = blockIdx.x;
+    const int chunk = rest % p.chunks;
+    rest /= p.chunks;
+    const int tile = rest % p.tiles;
+    rest /= p.tiles;
+    const int kvh = rest % p.kv_heads, seq = rest / p.kv_heads;
+    if (p.zero_tail && blockIdx.x == 0) {
+        const int64_t row = static_cast<int64_t>(p.q_heads) * D, used = p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs;
+        for (int64_t i = used * row + threadIdx.x; i < p.rows * row; i += kWarps * 32) static_cast<uint16_t*>(p.out)[i] = 0;
+    }
+    int first_row, nq;
+    const bool too_many = rows_of(p, seq, first_row, nq);
+    const int nrows = nq * p.group, r0 = tile * 8 * NT;
+    if (r0 >= nrows) return;
+    int len = p.seq_lens[seq];
+    const bool too_long = pages_of_length(len) > p.max_pages;
+    if (too_long) len = p.max_pages * kPageTokens;
+    if ((too_long || too_many) && p.status && threadIdx.x == 0 && chunk == 0 && tile == 0 && kvh == 0)
+        atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
+    Rows<D, NT> w;
+    load_queries<D, NT, BF16>(w, p, first_row, kvh, r0, nrows, len, nq, lane);
+    const int pages = pages_of_length(w.max_limit);
+    const int chunks = max((pages + p.chunk_pages - 1) / p.chunk_pages, 1);
+    if (chunk >= chunks) return;
+
+    const int c_a = chunk * p.chunk_pages, c_b = min(c_a + p.chunk_pages, pages);
+    const int share = (c_b - c_a + kWarps - 1) / kWarps;
+    const int a = c_a + warp * share, b = min(a + share, c_b);
+    const int32_t* table = p.tables + seq * p.table_stride;
+    bool bad = false;
+    auto address = [&](int page) {
+        int block = __ldg(table + page / p.pages_per_block);
+        if (block < 0 || block >= p.num_blocks) {
+            bad = true;
+            block = block < 0 ? 0 : static_cast<int>(p.num_blocks - 1);
+        }
+        return page_address<D>(p, page, block, kvh);
+    };
+    if (a < b) {
+        Page<D> x;
+        const uint8_t* base = address(a);
+        load_keys<D>(x, base, lane);
+        load_values<D>(x, base, lane);
+        for (int page = a; page < b; ++page) {
+            const bool more = page + 1 < b;
+            const uint8_t* next = more ? address(page + 1) : nullptr;
+            float s[NT][4];
+            uint32_t weights[NT][2];
+            page_scores<D, NT>(s, w, x);
+            const float2 scales = x.scales;
+            if (more) load_keys<D>(x, next, lane);
+            page_weights<D, NT>(w, s, scales, page, weights);
+            page_products<D, NT>(w, x, weights, page, lane);
+            if (more) load_values<D>(x, next, lane);
+        }
+    }
+    if (bad && p.status) atomicOr(p.status, TQ_STATUS_BAD_BLOCK);
+
+    // The warps' parts, with the values in units of the weights' reference.
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float l = w.l[n][j];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const int col = 8 * n + 2 * t + j;
+            const float up = ex2(w.u[n][j] - w.m[n][j] - kHeadroom);
+#pragma unroll
+            for (int i = 0; i < Rows<D, NT>::kSteps; ++i) {
+                part_o[warp][col][D / 8 * g + 2 * i] = w.o[i][n][j] * up;
+                part_o[warp][col][D / 8 * g + 2 * i + 1] = w.o[i][n][j + 2] * up;
+            }
+            if (g == 0) {
+                part_m[warp][col] = w.m[n][j];
+                part_l[warp][col] = l;
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * NT * D; i += kWarps * 32) {
+        const int col = i / D, d = i % D, row = r0 + col;
+        if (row >= nrows) break;
+        float m = kNothing, l = 0.f, o = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) m = fmaxf(m, part_m[k][col]);
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+            const float f = ex2(part_m[k][col] - m);
+            l += f * part_l[k][col];
+            o += f * part_o[k][col][d];
+        }
+        const int token = row / p.group, head = kvh * p.group + row - token * p.group;
+        const int64_t at = static_cast<int64_t>(first_row + token) * p.q_heads + head;
+        if (p.chunks == 1 || chunks == 1) {
+            store_out(p.out, at * D + d, l == 0.f ? 0.f : o / l, BF16);
+        } else {
+            float* to = p.partials + (at * p.chunks + chunk) * (D + 2);
+            to[d] = o;
+            if (d == 0) {
+                to[D] = m;
+                to[D + 1] = l;
+            }
+        }
+    }
+}
+
+// One warp per query row joins the parts of its chunks.
+template <int D>
+__global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params p, int bf16) {
+    pdl_release();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int seq = blockIdx.x / p.merge_blocks, r = (blockIdx.x - seq * p.merge_blocks) * 4 + (threadIdx.x >> 5);
+    int first_row, nq;
+    rows_of(p, seq, first_row, nq);
+    if (r >= nq * p.q_heads) return;
+    const int token = r / p.q_heads, head = r - token * p.q_heads, kvh = head / p.group, row = token * p.group + head - kvh * p.group;
+    const int len = min(p.seq_lens[seq], p.max_pages * kPageTokens);
+    const int last = min(row / p.tile_rows * p.tile_rows + p.tile_rows - 1, nq * p.group - 1);
+    const int pages = pages_of_length(len - nq + last / p.group + 1);
+    const int chunks = (pages + p.chunk_pages - 1) / p.chunk_pages;
+    if (chunks <= 1) return;                         // written by its only chunk
+    const int64_t at = static_cast<int64_t>(first_row + token) * p.q_heads + head;
+    const float* part = p.partials + at * p.chunks * (D + 2);
+    float m = kNothing;
+    for (int c = 0; c < chunks; ++c) m = fmaxf(m, part[c * (D + 2) + D]);
+    float l = 0.f, o[D / 32] = {};
+    for (int c = 0; c < chunks; ++c) {
+        const float f = ex2(part[c * (D + 2) + D] - m);
+        l += f * part[c * (D + 2) + D + 1];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] += f * part[c * (D + 2) + lane + 32 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) store_out(p.out, at * D + lane + 32 * i, l == 0.f ? 0.f : o[i] / l, bf16 != 0);
+}
+
+struct Attend8Plan {
+    int nt, tiles, chunk_pages, chunks;
+};
+
+Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
+    Attend8Plan a;
+    const int64_t rows = static_cast<int64_t>(group) * max_queries;
+    a.nt = rows <= 8 ? 1 : 2;
+    a.tiles = static_cast<int>((rows + 8 * a.nt - 1) / (8 * a.nt));
+    const int64_t items = seqs * kv_heads * a.tiles;
+    int64_t want = (148 * 4 + items - 1) / items;                       // chunks per item that fill the GPU
+    const int64_t most = (max_pages + 15) / 16;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    a.chunk_pages = static_cast<int>((max_pages + want - 1) / want);
+    if (a.chunk_pages < 1) a.chunk_pages = 1;
+    a.chunks = (max_pages + a.chunk_pages - 1) / a.chunk_pages;
+    if (a.chunks < 1) a.chunks = 1;
+    return a;
+}
+
+template <int D>
+cudaError_t launch_attend8(const Attend8Params& p, int nt, bool bf16, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs)), block(kWarps * 32);
+    cudaError_t err;
+    if (nt == 1) err = bf16 ? launch_chained(attend8_kernel<D, 1, true>, grid, block, 0, stream, p) : launch_chained(attend8_kernel<D, 1, false>, grid, block, 0, stream, p);
+    else err = bf16 ? launch_chained(attend8_kernel<D, 2, true>, grid, block, 0, stream, p) : launch_chained(attend8_kernel<D, 2, false>, grid, block, 0, stream, p);
+    if (err != cudaSuccess || p.chunks == 1) return err;
+    const dim3 merge(static_cast<unsigned>(p.merge_blocks) * p.seqs);
+    return launch_chained(attend8_merge_kernel<D>, merge, dim3(128), 0, stream, p, static_cast<int>(bf16));
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int64_t tq_attend8_workspace_bytes(int64_t num_rows, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int max_queries,
+                                              int max_pages_per_seq) {
+    using namespace tq;
+    if (num_rows < 0 || num_seqs < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads || max_queries < 1 || max_pages_per_seq < 0)
+        return TQ_ERR_ARG;
+    if (head_dim != 64 && head_dim != 128) return TQ_ERR_UNSUPPORTED;
+    if (num_seqs == 0) return 0;
+    const Attend8Plan a = attend8_plan(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
+    return a.chunks == 1 ? 0 : num_rows * num_q_heads * a.chunks * (head_dim + 2) * 4;
+}
+
+extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const void* cache, int64_t num_blocks, int block_size,
+                                const int32_t* block_tables, int64_t bt_stride, const int32_t* seq_lens, const int32_t* query_start_loc,
+                                float sm_scale, void* workspace, int64_t workspace_bytes, int32_t* status, int64_t num_rows, int num_seqs,
+                                int num_q_heads, int num_kv_heads, int head_dim, int max_queries, int max_pages_per_seq, int zero_tail,
+                                tq_stream_t stream) {
+    using namespace tq;
+    if (num_rows < 0 || num_seqs < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads || num_blocks < 0 || max_queries < 1 ||
+        max_pages_per_seq < 0 || bt_stride < 0)
+        return TQ_ERR_ARG;
+    if ((io_dtype != TQ_DTYPE_F16 && io_dtype != TQ_DTYPE_BF16) || (head_dim != 64 && head_dim != 128)) return TQ_ERR_UNSUPPORTED;
+    if (block_size < kPageTokens || block_size % kPageTokens || num_blocks > INT32_MAX || num_rows > INT32_MAX) return TQ_ERR_UNSUPPORTED;
+    if (max_pages_per_seq > (1 << 27) - 1 || static_cast<int64_t>(max_queries) * num_q_heads > (1 << 30)) return TQ_ERR_UNSUPPORTED;
+    if (num_rows == 0) return TQ_OK;
+    if (num_seqs == 0) {
+        if (!zero_tail) return TQ_OK;
+        if (!out) return TQ_ERR_ARG;
+        return cudaMemsetAsync(out, 0, static_cast<size_t>(num_rows) * num_q_heads * head_dim * 2, stream) == cudaSuccess ? TQ_OK : TQ_ERR_LAUNCH;
+    }
+    if (!out || !q || !cache || !block_tables || !seq_lens || num_blocks == 0) return TQ_ERR_ARG;
+    if (!query_start_loc && (num_rows < num_seqs || max_queries != 1)) return TQ_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) % 16) return TQ_ERR_ARG;
+    const Attend8Plan a = attend8_plan(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
+    const int64_t merge_blocks = (static_cast<int64_t>(max_queries) * num_q_heads + 3) / 4;
+    if (static_cast<double>(num_kv_heads) * a.tiles * a.chunks * num_seqs > INT32_MAX || static_cast<double>(merge_blocks) * num_seqs > INT32_MAX)
+        return TQ_ERR_UNSUPPORTED;
+    const int64_t need = a.chunks == 1 ? 0 : num_rows * num_q_heads * a.chunks * (head_dim + 2) * 4;
+    if (need && (!workspace || workspace_bytes < need)) return TQ_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return TQ_ERR_ARG;
+    Attend8Params p = {};
+    p.out = out; p.q = q; p.cache = static_cast<const uint8_t*>(cache); p.tables = block_tables; p.seq_lens = seq_lens; p.starts = query_start_loc;
+    p.partials = static_cast<float*>(workspace); p.status = status; p.num_blocks = num_blocks; p.table_stride = bt_stride;
+    p.scale_log2 = sm_scale * kLog2e; p.rows = static_cast<int>(num_rows); p.seqs = num_seqs; p.q_heads = num_q_heads; p.kv_heads = num_kv_heads;
+    p.group = num_q_heads / num_kv_heads; p.pages_per_block = block_size / kPageTokens; p.max_pages = max_pages_per_seq; p.max_queries = max_queries;
+    p.tiles = a.tiles; p.tile_rows = 8 * a.nt; p.merge_blocks = static_cast<int>(merge_blocks); p.chunk_pages = a.chunk_pages; p.chunks = a.chunks; p.zero_tail = zero_tail;
+    const cudaError_t err = head_dim == 64 ? launch_attend8<64>(p, a.nt, io_dtype == TQ_DTYPE_BF16, stream)
+                                           : launch_attend8<128>(p, a.nt, io_dtype == TQ_DTYPE_BF16, stream);
+    return err == cudaSuccess ? TQ_OK : TQ_ERR_LAUNCH;
+}

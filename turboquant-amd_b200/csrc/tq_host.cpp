@@ -40,6 +40,13 @@ struct Library {
     decltype(&tq_polarquant_compress) polarquant;
     decltype(&tq_packed_attention_workspace_bytes) attention_workspace_bytes;
     decltype(&tq_packed_attention) packed_attention;
+    decltype(&tq_rotary) rotary;
+    decltype(&tq_cache8_page_bytes) cache8_page_bytes;
+    decltype(&tq_quantize8_paged) quantize8_paged;
+    decltype(&tq_attend8_workspace_bytes) attend8_workspace_bytes;
+    decltype(&tq_attend8_paged) attend8_paged;
+    decltype(&tq_plan_step) plan_step;
+    decltype(&tq_release_blocks) release_blocks;
 };
 Library L = {};
 
@@ -395,6 +402,222 @@ PyObject* packed_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // as the custom op's schema says
+}
+
+// The device's status word, or null while there is none (the general path makes it).
+int32_t* status_of(const at::Tensor& t) {
+    const int dev = t.get_device();
+    return dev >= 0 && dev < kMaxDevices ? g_status[dev] : nullptr;
+}
+
+bool is_vector(const at::Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.dim() == 1 && t.is_contiguous(); }
+
+bool is_table(const at::Tensor& t, int64_t rows) {
+    return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) >= rows && (t.size(1) <= 1 || t.stride(1) == 1);
+}
+
+// uint8 [blocks, heads, block_size / 16 * page bytes] for heads of dim values
+bool is_cache8(const at::Tensor& t, long long block_size, int64_t dim) {
+    return (dim == 64 || dim == 128) && block_size >= 16 && block_size % 16 == 0 && block_size <= 1 << 20 && t.scalar_type() == at::kByte &&
+           t.dim() == 3 && t.is_contiguous() && t.size(2) == block_size / 16 * L.cache8_page_bytes(int(dim));
+}
+
+uintptr_t address(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); }
+
+// rotary(q, k | None, positions, cos_sin, interleaved, inverse) -> (q, k | None)
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 6 || !plain_eager()) return declined();
+    const bool has_k = args[1] != Py_None;
+    PyObject* const in[4] = {args[0], has_k ? args[1] : args[0], args[2], args[3]};
+    const at::Tensor* t[4];
+    long long v[2];
+    if (!tensors_on_one_device(in, t) || !ints(args + 4, 2, v)) return declined();
+    const at::Tensor &q = *t[0], &k = *t[1], &positions = *t[2], &table = *t[3];
+    int32_t* status = status_of(q);
+    const int dtype = dtype_code(q);
+    if (!status || dtype < 0 || q.dim() != 3 || q.stride(2) != 1 || k.dim() != 3 || k.stride(2) != 1 || k.scalar_type() != q.scalar_type() ||
+        k.size(0) != q.size(0) || k.size(2) != q.size(2))
+        return declined();
+    const int64_t T = q.size(0), dim = q.size(2);
+    const bool wide = positions.scalar_type() == at::kLong;
+    if ((!wide && positions.scalar_type() != at::kInt) || positions.dim() != 1 || !positions.is_contiguous() || positions.numel() != T) return declined();
+    if (table.scalar_type() != at::kFloat || table.dim() != 2 || !table.is_contiguous() || table.size(0) < 1 || table.size(1) < 2 ||
+        table.size(1) % 2 || table.size(1) > dim || dim > 1 << 20)
+        return declined();
+    const at::Device dev = q.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor q_out = empty(q.sizes(), q.scalar_type(), dev), k_out;
+    if (has_k) k_out = empty(k.sizes(), k.scalar_type(), dev);
+    const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), q.size(1) * dim, dim, k.size(1) * dim, dim};
+    const tq_stream_t stream = stream_of(dev);
+    const int rc = launch([&] {
+        return L.rotary(q.data_ptr(), has_k ? k.data_ptr() : nullptr, q_out.data_ptr(), has_k ? k_out.data_ptr() : nullptr, dtype, strides,
+                        positions.data_ptr(), wide, table.data_ptr<float>(), table.size(0), T, int(std::min<int64_t>(q.size(1), INT32_MAX)),
+                        has_k ? int(std::min<int64_t>(k.size(1), INT32_MAX)) : 0, int(dim), int(table.size(1)), v[0] != 0, v[1] != 0, status,
+                        stream);
+    });
+    if (rc != TQ_OK) return failed("tq_rotary", rc);
+    if (!has_k) return Py_BuildValue("(NO)", THPVariable_Wrap(std::move(q_out)), Py_None);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(q_out)), THPVariable_Wrap(std::move(k_out)));
+    END_HANDLE_TH_ERRORS
+}
+
+// quantize8(key, value, cache, slot_mapping, block_size) -> True
+PyObject* quantize8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const at::Tensor* t[4];
+    long long block_size;
+    if (nargs != 5 || !plain_eager() || !tensors_on_one_device(args, t) || !ints(args + 4, 1, &block_size)) return declined();
+    const at::Tensor &key = *t[0], &value = *t[1], &cache = *t[2], &slots = *t[3];
+    int32_t* status = status_of(key);
+    const int dtype = dtype_code(key);
+    if (!status || dtype < 0 || key.dim() != 3 || value.scalar_type() != key.scalar_type() || value.sizes() != key.sizes() || key.stride(2) != 1 ||
+        value.stride(2) != 1)
+        return declined();
+    const int64_t T = key.size(0), H = key.size(1), dim = key.size(2);
+    if (!is_cache8(cache, block_size, dim) || cache.size(1) != H || H > INT32_MAX) return declined();
+    if (slots.scalar_type() != at::kLong || slots.numel() < T || !slots.is_contiguous()) return declined();
+    for (const at::Tensor* x : {&key, &value}) {     // rows are read 16 bytes at a time: others are copied
+        if ((address(*x) | static_cast<uint64_t>((x->stride(0) | x->stride(1)) * x->element_size())) % 16) return declined();
+    }
+    const c10::cuda::CUDAGuard guard(key.device());
+    const tq_stream_t stream = stream_of(key.device());
+    const int rc = launch([&] {
+        return L.quantize8_paged(key.data_ptr(), value.data_ptr(), dtype, key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+                                 cache.data_ptr(), cache.size(0), int(block_size), slots.data_ptr<int64_t>(), T, int(H), int(dim), status, stream);
+    });
+    if (rc != TQ_OK) return failed("tq_quantize8_paged", rc);
+    written(cache);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// attend8(q, cache, block_tables, seq_lens, query_start_loc | None, out | None, sm_scale, block_size, max_query_len, max_seq_len) -> out
+PyObject* attend8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const at::Tensor* t[4];
+    float scale[1];
+    long long v[3];
+    if (nargs != 10 || !plain_eager() || !tensors_on_one_device(args, t) || !floats(args + 6, 1, scale) || !ints(args + 7, 3, v)) return declined();
+    const at::Tensor &q = *t[0], &cache = *t[1], &tables = *t[2], &lens = *t[3];
+    int32_t* status = status_of(q);
+    const long long block_size = v[0], max_queries = v[1], max_len = v[2];
+    const int dtype = dtype_code(q);
+    if (!status || (dtype != TQ_DTYPE_F16 && dtype != TQ_DTYPE_BF16) || q.dim() != 3 || !q.is_contiguous() || address(q) % 16) return declined();
+    const int64_t T = q.size(0), hq = q.size(1), dim = q.size(2);
+    if (!is_cache8(cache, block_size, dim)) return declined();
+    const int64_t hkv = cache.size(1);
+    if (hkv < 1 || hq < 1 || hq % hkv || cache.size(0) < 1 || hq > INT32_MAX || max_queries < 1 || max_queries > INT32_MAX) return declined();
+    int64_t ns = T;
+    const int32_t* starts = nullptr;
+    auto other = [&](PyObject* obj) -> const at::Tensor* {
+        const at::Tensor* x = cuda_tensor(obj);
+        return !x || x->get_device() != q.get_device() || (x->requires_grad() && at::GradMode::is_enabled()) ? nullptr : x;
+    };
+    if (args[4] != Py_None) {
+        const at::Tensor* x = other(args[4]);
+        if (!x || !is_vector(*x, at::kInt) || x->numel() < 1) return declined();
+        ns = x->numel() - 1;
+        starts = x->data_ptr<int32_t>();
+    } else if (max_queries != 1) {
+        return declined();
+    }
+    if (ns > INT32_MAX || !is_table(tables, ns) || lens.scalar_type() != at::kInt || !lens.is_contiguous() || lens.numel() < ns) return declined();
+    void* out_ptr = nullptr;
+    if (args[5] != Py_None) {
+        const at::Tensor* x = other(args[5]);
+        if (!x || x->sizes() != q.sizes() || x->scalar_type() != q.scalar_type() || !x->is_contiguous()) return declined();
+        out_ptr = x->data_ptr();
+    }
+    int64_t pages = tables.size(1) * (block_size / 16);
+    if (max_len > 0) pages = std::min<int64_t>(pages, (max_len + 15) / 16);
+    if (pages > INT32_MAX) return declined();
+    const at::Device dev = q.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor out;
+    if (!out_ptr) {
+        out = empty(q.sizes(), q.scalar_type(), dev);
+        out_ptr = out.data_ptr();
+    }
+    const int64_t bytes = L.attend8_workspace_bytes(T, int(ns), int(hq), int(hkv), int(dim), int(max_queries), int(pages));
+    if (bytes < 0) return failed("tq_attend8_paged", int(bytes));
+    at::DataPtr workspace;      // this call's own: see decode()
+    if (bytes) workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+    const tq_stream_t stream = stream_of(dev);
+    const int rc = launch([&] {
+        return L.attend8_paged(out_ptr, q.data_ptr(), dtype, cache.data_ptr(), cache.size(0), int(block_size), tables.data_ptr<int32_t>(),
+                               tables.stride(0), lens.data_ptr<int32_t>(), starts, scale[0], workspace.get(), bytes, status, T, int(ns),
+                               int(hq), int(hkv), int(dim), int(max_queries), int(pages), out.defined(), stream);
+    });
+    if (rc != TQ_OK) return failed("tq_attend8_paged", rc);
+    if (out.defined()) return THPVariable_Wrap(std::move(out));
+    written(THPVariable_Unpack(args[5]));
+    Py_INCREF(args[5]);
+    return args[5];
+    END_HANDLE_TH_ERRORS
+}
+
+// plan_step(query_lens, context_lens, block_tables, free_blocks, free_count, block_size, num_rows)
+//   -> (slot_mapping, positions, seq_lens, query_start_loc, free_count)
+PyObject* plan_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const at::Tensor* t[5];
+    long long v[2];
+    if (nargs != 7 || !plain_eager() || !tensors_on_one_device(args, t) || !ints(args + 5, 2, v)) return declined();
+    const at::Tensor &query = *t[0], &context = *t[1], &tables = *t[2], &stack = *t[3], &count = *t[4];
+    int32_t* status = status_of(query);
+    const int64_t n = query.numel();
+    if (!status || !is_vector(query, at::kInt) || !is_vector(context, at::kInt) || context.numel() != n || !is_table(tables, n) ||
+        !is_vector(stack, at::kInt) || !is_vector(count, at::kInt) || count.numel() != 1 || v[0] < 1 || v[0] > INT32_MAX || v[1] < 0)
+        return declined();
+    const at::Device dev = query.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor slots = empty({v[1]}, at::kLong, dev), positions = empty({v[1]}, at::kLong, dev), lens = empty({n}, at::kInt, dev);
+    at::Tensor starts = empty({n + 1}, at::kInt, dev), left = empty({1}, at::kInt, dev);
+    const tq_stream_t stream = stream_of(dev);
+    const int rc = launch([&] {
+        return L.plan_step(query.data_ptr<int32_t>(), context.data_ptr<int32_t>(), tables.data_ptr<int32_t>(), tables.stride(0),
+                           stack.data_ptr<int32_t>(), count.data_ptr<int32_t>(), slots.data_ptr<int64_t>(), positions.data_ptr<int64_t>(),
+                           lens.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), left.data_ptr<int32_t>(), status, n, tables.size(1),
+                           stack.numel(), int(v[0]), v[1], stream);
+    });
+    if (rc != TQ_OK) return failed("tq_plan_step", rc);
+    written(tables);
+    return Py_BuildValue("(NNNNN)", THPVariable_Wrap(std::move(slots)), THPVariable_Wrap(std::move(positions)),
+                         THPVariable_Wrap(std::move(lens)), THPVariable_Wrap(std::move(starts)), THPVariable_Wrap(std::move(left)));
+    END_HANDLE_TH_ERRORS
+}
+
+// release_blocks(ended, context_lens, block_tables, free_blocks, free_count, block_size) -> (context_lens, free_count)
+PyObject* release_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const at::Tensor* t[5];
+    long long block_size;
+    if (nargs != 6 || !plain_eager() || !tensors_on_one_device(args, t) || !ints(args + 5, 1, &block_size)) return declined();
+    const at::Tensor &ended = *t[0], &context = *t[1], &tables = *t[2], &stack = *t[3], &count = *t[4];
+    int32_t* status = status_of(ended);
+    const int64_t n = ended.numel();
+    if (!status || !is_vector(ended, at::kBool) || !is_vector(context, at::kInt) || context.numel() != n || !is_table(tables, n) ||
+        !is_vector(stack, at::kInt) || !is_vector(count, at::kInt) || count.numel() != 1 || block_size < 1 || block_size > INT32_MAX)
+        return declined();
+    const at::Device dev = ended.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor lens = empty({n}, at::kInt, dev), left = empty({1}, at::kInt, dev);
+    const tq_stream_t stream = stream_of(dev);
+    const int rc = launch([&] {
+        return L.release_blocks(reinterpret_cast<const uint8_t*>(ended.data_ptr<bool>()), context.data_ptr<int32_t>(), tables.data_ptr<int32_t>(),
+                                tables.stride(0), stack.data_ptr<int32_t>(), count.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+                                left.data_ptr<int32_t>(), status, n, tables.size(1), stack.numel(), int(block_size), stream);
+    });
+    if (rc != TQ_OK) return failed("tq_release_blocks", rc);
+    written(stack);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(lens)), THPVariable_Wrap(std::move(left)));
+    END_HANDLE_TH_ERRORS
+}
+
 // set_status(device index, int32 tensor that lives as long as the process)
 PyObject* set_status(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
@@ -436,6 +659,13 @@ PyObject* bind(PyObject*, PyObject* args) {
     take(L.polarquant, "tq_polarquant_compress");
     take(L.attention_workspace_bytes, "tq_packed_attention_workspace_bytes");
     take(L.packed_attention, "tq_packed_attention");
+    take(L.rotary, "tq_rotary");
+    take(L.cache8_page_bytes, "tq_cache8_page_bytes");
+    take(L.quantize8_paged, "tq_quantize8_paged");
+    take(L.attend8_workspace_bytes, "tq_attend8_workspace_bytes");
+    take(L.attend8_paged, "tq_attend8_paged");
+    take(L.plan_step, "tq_plan_step");
+    take(L.release_blocks, "tq_release_blocks");
     if (!ok) {
         PyErr_Format(PyExc_RuntimeError, "%s lacks a tq_* entry point", path);
         return nullptr;
@@ -454,6 +684,11 @@ PyMethodDef kMethods[] = {
     {"compress_v", fast<compress_v>(), METH_FASTCALL, nullptr},
     {"polarquant", fast<polarquant>(), METH_FASTCALL, nullptr},
     {"packed_attention", fast<packed_attention>(), METH_FASTCALL, nullptr},
+    {"rotary", fast<rotary>(), METH_FASTCALL, nullptr},
+    {"quantize8", fast<quantize8>(), METH_FASTCALL, nullptr},
+    {"attend8", fast<attend8>(), METH_FASTCALL, nullptr},
+    {"plan_step", fast<plan_step>(), METH_FASTCALL, nullptr},
+    {"release_blocks", fast<release_blocks>(), METH_FASTCALL, nullptr},
     {"set_status", set_status, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -13,6 +13,11 @@ Ops registered (namespace `tq_b200`):
   decode_paged(q_rot, q_proj, cache, block_tables, seq_lens, kc, vc, sm_scale, corr_scale, sparse_thresh,
                block_size, k_bits, v_bits, use_qjl, chunk_pages, io_flags, max_seq_len) -> out
   wht_rows(x, scale) -> x @ H * scale
+  rotary(q, k, positions, cos_sin, interleaved, inverse) -> (q, k)
+  quantize8_paged(key, value, cache, slot_mapping, block_size)
+  attend8_paged(q, cache, block_tables, seq_lens, query_start_loc, sm_scale, block_size, max_query_len, max_seq_len) -> out
+  plan_step(query_lens, context_lens, block_tables, free_blocks, free_count, block_size, num_rows) -> 5 tensors
+  release_blocks(ended, context_lens, block_tables, free_blocks, free_count, block_size) -> (context_lens, free_count)
 """
 from __future__ import annotations
 
@@ -29,6 +34,9 @@ _ERRORS = {-1: "bad argument", -2: "unsupported configuration", -3: "CUDA launch
 STATUS_BAD_BLOCK = 1
 STATUS_TIMEOUT = 2
 STATUS_BAD_SLOT = 4
+STATUS_BAD_POSITION = 8
+STATUS_NO_BLOCKS = 16
+STATUS_TOO_LONG = 32
 IO_ROTATE_Q = 0x100        # q is in original space: rotate it inside the decode kernel
 IO_DEROTATE_OUT = 0x200    # write the decode output in original space
 IO_TCGEN05 = 0x400         # tensor-memory variant of the decode kernel (2- / 3-bit codebooks, no Sparse-V)
@@ -77,7 +85,16 @@ def lib() -> ctypes.CDLL:
     L.tq_packed_attention_workspace_bytes.restype = i64
     L.tq_packed_attention_auto_splits.argtypes = [i32, i32]
     L.tq_packed_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32, i32, i32, i32, vp, i64, vp, vp]
-    for name in ("tq_page_bytes", "tq_compress_paged", "tq_decode_auto_chunk_pages", "tq_decode_paged",
+    L.tq_rotary.argtypes = [vp, vp, vp, vp, i32, ctypes.POINTER(i64), vp, i32, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, vp]
+    L.tq_cache8_page_bytes.argtypes = [i32]
+    L.tq_quantize8_paged.argtypes = [vp, vp, i32, i64, i64, i64, i64, vp, i64, i32, vp, i64, i32, i32, vp, vp]
+    L.tq_attend8_workspace_bytes.argtypes = [i64, i32, i32, i32, i32, i32, i32]
+    L.tq_attend8_workspace_bytes.restype = i64
+    L.tq_attend8_paged.argtypes = [vp, vp, i32, vp, i64, i32, vp, i64, vp, vp, f32, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, i32, vp]
+    L.tq_plan_step.argtypes = [vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, i64, vp]
+    L.tq_release_blocks.argtypes = [vp, vp, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]
+    for name in ("tq_rotary", "tq_cache8_page_bytes", "tq_quantize8_paged", "tq_attend8_paged", "tq_plan_step", "tq_release_blocks",
+                 "tq_page_bytes", "tq_compress_paged", "tq_decode_auto_chunk_pages", "tq_decode_paged",
                  "tq_decode_paged_static", "tq_wht_rows", "tq_compress_k", "tq_compress_v", "tq_polarquant_compress",
                  "tq_packed_attention_auto_splits", "tq_packed_attention"):
         getattr(L, name).restype = i32
@@ -332,6 +349,170 @@ def polarquant(x: torch.Tensor, centroids, boundaries, bits: int, use_qjl: bool,
     return res
 
 
+def _rotary_impl(q, k, q_out, k_out, positions, cos_sin, interleaved: bool, inverse: bool) -> None:
+    dev = _require_cuda(q, k, q_out, k_out, positions, cos_sin)
+    if q.dim() != 3 or q.dtype not in _DTYPES:
+        raise ValueError("q must be [tokens, heads, head_dim] in fp16, bf16 or fp32")
+    T, _, D = q.shape
+    for name, t, like in (("q_out", q_out, q), ("k", k, None), ("k_out", k_out, k)):
+        if name == "k_out" and (t is None) != (k is None):
+            raise ValueError("k and its output go together")
+        if t is None:
+            continue
+        if t.dtype != q.dtype or (like is not None and t.shape != like.shape) or t.dim() != 3 or t.shape[0] != T or t.shape[2] != D:
+            raise ValueError(f"{name} must match in dtype, tokens and head_dim, an output its input in shape")
+    for t in (q, k, q_out, k_out):
+        if t is not None and t.stride(-1) != 1:
+            raise ValueError("the head dimension must be contiguous")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.shape[0] < 1:
+        raise ValueError("cos_sin must be contiguous fp32 [positions, rotary_dim]")
+    R = cos_sin.shape[1]
+    if R < 2 or R % 2 or R > D:
+        raise ValueError("rotary_dim must be even and at most head_dim")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.numel() != T or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 or int64 with one entry per token")
+    zero = (0, 0)
+    st = (ctypes.c_int64 * 8)(*q.stride()[:2], *(k.stride()[:2] if k is not None else zero), *q_out.stride()[:2],
+                              *(k_out.stride()[:2] if k is not None else zero))
+    with torch.cuda.device(dev):
+        rc = lib().tq_rotary(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _DTYPES[q.dtype], st, _ptr(positions),
+                             int(positions.dtype == torch.int64), _ptr(cos_sin), cos_sin.shape[0], T, q.shape[1],
+                             0 if k is None else k.shape[1], D, R, int(interleaved), int(inverse), _ptr(status_word(dev)), _stream(dev))
+    _check(rc, "tq_rotary")
+
+
+def _quantize8_impl(key, value, cache, slot_mapping, block_size: int) -> None:
+    dev = _require_cuda(key, value, cache, slot_mapping)
+    if key.dim() != 3 or key.shape[-1] not in (64, 128) or value.shape != key.shape:
+        raise ValueError("key/value must be [tokens, kv_heads, 64 or 128]")
+    if key.dtype not in _DTYPES or value.dtype != key.dtype:
+        raise ValueError("key/value must share a dtype of fp16, bf16 or fp32")
+    if key.stride(-1) != 1 or value.stride(-1) != 1:
+        raise ValueError("the head dimension must be contiguous")
+    T, H, D = key.shape
+    _check_cache8(cache, block_size, D)
+    if cache.shape[1] != H:
+        raise ValueError("cache and key differ in their number of heads")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < T or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int64 with at least one entry per token")
+    key, value = (t if _aligned_rows(t) else t.contiguous().clone() for t in (key, value))      # rows are read 16 bytes at a time
+    with torch.cuda.device(dev):
+        rc = lib().tq_quantize8_paged(
+            _ptr(key), _ptr(value), _DTYPES[key.dtype], key.stride(0), key.stride(1), value.stride(0), value.stride(1), _ptr(cache),
+            cache.shape[0], block_size, _ptr(slot_mapping), T, H, D, _ptr(status_word(dev)), _stream(dev))
+    _check(rc, "tq_quantize8_paged")
+
+
+def _aligned_rows(t: torch.Tensor) -> bool:
+    return (t.data_ptr() | (t.stride(0) | t.stride(1)) * t.element_size()) % 16 == 0
+
+
+def _check_cache8(cache: torch.Tensor, block_size: int, head_dim: int) -> None:
+    if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous():
+        raise ValueError("cache must be a contiguous uint8 [num_blocks, kv_heads, bytes] tensor")
+    expected = block_size // 16 * lib().tq_cache8_page_bytes(head_dim)
+    if block_size < 16 or block_size % 16 or cache.shape[2] != expected:
+        raise ValueError(f"cache row of {cache.shape[2]} bytes does not match block_size {block_size} and head_dim {head_dim} "
+                         f"({expected} expected)")
+
+
+def _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_scale: float, block_size: int, max_query_len: int,
+                  max_seq_len: int, zero_tail: bool) -> None:
+    dev = _require_cuda(out, q, cache, block_tables, seq_lens, query_start_loc)
+    if q.dim() != 3 or q.shape[-1] not in (64, 128) or not q.is_contiguous():
+        raise ValueError("q must be contiguous [tokens, q_heads, 64 or 128]")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("q must be fp16 or bf16")
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must match q in shape and dtype and be contiguous")
+    T, Hq, D = q.shape
+    _check_cache8(cache, block_size, D)
+    nb, Hkv, _ = cache.shape
+    if Hq < 1 or Hkv < 1 or Hq % Hkv:
+        raise ValueError("q heads must be a multiple of kv heads")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [num_seqs, max_blocks] with contiguous rows")
+    if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous int32 [num_seqs]")
+    if query_start_loc is None:
+        ns = T
+        if max_query_len != 1:
+            raise ValueError("several query tokens per sequence need query_start_loc")
+    else:
+        if query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1 or not query_start_loc.is_contiguous() or query_start_loc.numel() < 1:
+            raise ValueError("query_start_loc must be contiguous int32 [num_seqs + 1]")
+        ns = query_start_loc.numel() - 1
+    if max_query_len < 1:
+        raise ValueError("max_query_len must be positive")
+    if seq_lens.numel() < ns or block_tables.shape[0] < ns:
+        raise ValueError("seq_lens and block_tables need an entry for every sequence")
+    if T and ns and nb < 1:
+        raise ValueError("the cache has no blocks")
+    max_pages = block_tables.shape[1] * (block_size // 16)
+    if max_seq_len > 0:
+        max_pages = min(max_pages, (int(max_seq_len) + 15) // 16)
+    L = lib()
+    if q.data_ptr() % 16:
+        q = q.clone()                                             # read 16 bytes at a time
+    with torch.cuda.device(dev):
+        need = L.tq_attend8_workspace_bytes(T, ns, Hq, Hkv, D, max_query_len, max_pages)
+        if need < 0:
+            _check(need, "tq_attend8_workspace_bytes")
+        ws = workspace(dev, need)
+        rc = L.tq_attend8_paged(_ptr(out), _ptr(q), _DTYPES[q.dtype], _ptr(cache), nb, block_size, _ptr(block_tables), block_tables.stride(0),
+                                _ptr(seq_lens), _ptr(query_start_loc), float(sm_scale), _ptr(ws), ws.numel(), _ptr(status_word(dev)), T, ns,
+                                Hq, Hkv, D, int(max_query_len), max_pages, int(zero_tail), _stream(dev))
+    _check(rc, "tq_attend8_paged")
+
+
+def _check_requests(lens, block_tables, free_blocks, free_count, block_size: int) -> int:
+    n = lens[0].numel()
+    for t in (*lens, free_blocks, free_count):
+        if t.dim() != 1 or not t.is_contiguous():
+            raise ValueError("lengths, free_blocks and free_count must be contiguous vectors")
+    if any(t.dtype != torch.int32 for t in (*lens[-1:], block_tables, free_blocks, free_count)):
+        raise ValueError("context_lens, block_tables, free_blocks and free_count must be int32")
+    if any(t.numel() != n for t in lens) or block_tables.dim() != 2 or block_tables.shape[0] < n or free_count.numel() != 1:
+        raise ValueError("one length and one row of block_tables per request, free_count of one element")
+    if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
+        raise ValueError("block_tables must have contiguous rows")
+    if block_size < 1:
+        raise ValueError("block_size must be positive")
+    return n
+
+
+def _plan_step_impl(query_lens, context_lens, block_tables, free_blocks, free_count, block_size: int, num_rows: int):
+    dev = _require_cuda(query_lens, context_lens, block_tables, free_blocks, free_count)
+    if query_lens.dtype != torch.int32:
+        raise ValueError("query_lens must be int32")
+    n = _check_requests((query_lens, context_lens), block_tables, free_blocks, free_count, block_size)
+    if num_rows < 0:
+        raise ValueError("num_rows must not be negative")
+    wide = lambda m: torch.empty(m, dtype=torch.int64, device=dev)
+    ints = lambda m: torch.empty(m, dtype=torch.int32, device=dev)
+    slots, positions, seq_lens, starts, count = wide(num_rows), wide(num_rows), ints(n), ints(n + 1), ints(1)
+    with torch.cuda.device(dev):
+        rc = lib().tq_plan_step(_ptr(query_lens), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0), _ptr(free_blocks),
+                                _ptr(free_count), _ptr(slots), _ptr(positions), _ptr(seq_lens), _ptr(starts), _ptr(count),
+                                _ptr(status_word(dev)), n, block_tables.shape[1], free_blocks.numel(), block_size, num_rows, _stream(dev))
+    _check(rc, "tq_plan_step")
+    return slots, positions, seq_lens, starts, count
+
+
+def _release_blocks_impl(ended, context_lens, block_tables, free_blocks, free_count, block_size: int):
+    dev = _require_cuda(ended, context_lens, block_tables, free_blocks, free_count)
+    if ended.dtype != torch.bool:
+        raise ValueError("ended must be bool")
+    n = _check_requests((ended, context_lens), block_tables, free_blocks, free_count, block_size)
+    lens, count = torch.empty_like(context_lens), torch.empty_like(free_count)
+    with torch.cuda.device(dev):
+        rc = lib().tq_release_blocks(_ptr(ended), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0), _ptr(free_blocks),
+                                     _ptr(free_count), _ptr(lens), _ptr(count), _ptr(status_word(dev)), n, block_tables.shape[1],
+                                     free_blocks.numel(), block_size, _stream(dev))
+    _check(rc, "tq_release_blocks")
+    return lens, count
+
+
 # ---- torch custom ops --------------------------------------------------------------------------
 @torch.library.custom_op("tq_b200::compress_paged", mutates_args=("cache",))
 def compress_paged_op(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -373,3 +554,68 @@ def wht_rows_op(x: torch.Tensor, scale: float) -> torch.Tensor:
 @wht_rows_op.register_fake
 def _(x, scale):
     return torch.empty_like(x)
+
+
+@torch.library.custom_op("tq_b200::rotary", mutates_args=())
+def rotary_op(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool,
+              inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _require_cuda(q, k, positions, cos_sin)
+    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    q_out = new(q)
+    k_out = new(k) if k is not None else q.new_empty(0)
+    _rotary_impl(q, k, q_out, k_out if k is not None else None, positions, cos_sin, interleaved, inverse)
+    return q_out, k_out
+
+
+@rotary_op.register_fake
+def _(q, k, positions, cos_sin, interleaved, inverse):
+    return q.new_empty(q.shape), (k.new_empty(k.shape) if k is not None else q.new_empty(0))
+
+
+@torch.library.custom_op("tq_b200::quantize8_paged", mutates_args=("cache",))
+def quantize8_paged_op(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, slot_mapping: torch.Tensor, block_size: int) -> None:
+    _quantize8_impl(key, value, cache, slot_mapping, block_size)
+
+
+@quantize8_paged_op.register_fake
+def _(key, value, cache, slot_mapping, block_size) -> None:
+    return None
+
+
+@torch.library.custom_op("tq_b200::attend8_paged", mutates_args=())
+def attend8_paged_op(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                     query_start_loc: Optional[torch.Tensor], sm_scale: float, block_size: int, max_query_len: int,
+                     max_seq_len: int) -> torch.Tensor:
+    out = torch.empty_like(q)
+    _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_scale, block_size, max_query_len, max_seq_len, zero_tail=True)
+    return out
+
+
+@attend8_paged_op.register_fake
+def _(q, cache, block_tables, seq_lens, query_start_loc, sm_scale, block_size, max_query_len, max_seq_len):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op("tq_b200::plan_step", mutates_args=("block_tables",))
+def plan_step_op(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, free_blocks: torch.Tensor,
+                 free_count: torch.Tensor, block_size: int,
+                 num_rows: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _plan_step_impl(query_lens, context_lens, block_tables, free_blocks, free_count, block_size, num_rows)
+
+
+@plan_step_op.register_fake
+def _(query_lens, context_lens, block_tables, free_blocks, free_count, block_size, num_rows):
+    n, wide = query_lens.numel(), dict(dtype=torch.int64)
+    return (query_lens.new_empty(num_rows, **wide), query_lens.new_empty(num_rows, **wide), query_lens.new_empty(n),
+            query_lens.new_empty(n + 1), query_lens.new_empty(1))
+
+
+@torch.library.custom_op("tq_b200::release_blocks", mutates_args=("free_blocks",))
+def release_blocks_op(ended: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, free_blocks: torch.Tensor,
+                      free_count: torch.Tensor, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _release_blocks_impl(ended, context_lens, block_tables, free_blocks, free_count, block_size)
+
+
+@release_blocks_op.register_fake
+def _(ended, context_lens, block_tables, free_blocks, free_count, block_size):
+    return torch.empty_like(context_lens), torch.empty_like(free_count)

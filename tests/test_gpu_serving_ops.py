@@ -253,8 +253,10 @@ def _filled(g, lens, H, D, bs, spread=3):
     return cache, tables.to(DEV)
 
 
-def _check_attention(g, lens, queries, Hq, H, D, bs, dtype, sm_scale=None, q_size=1.0, spread=3, **call):
+def _check_attention(g, lens, queries, Hq, H, D, bs, dtype, sm_scale=None, q_size=1.0, spread=3, width=0, **call):
     cache, tables = _filled(g, lens, H, D, bs, spread)
+    if width > tables.shape[1]:                                             # launches are sized for the table where nothing else is said
+        tables = torch.nn.functional.pad(tables, (0, width - tables.shape[1]), value=-9)
     T = sum(queries)
     q = (torch.randn(T, Hq, D, generator=g, device=DEV) * q_size).to(dtype)
     starts = np.concatenate([[0], np.cumsum(queries)])
@@ -297,6 +299,32 @@ def test_several_queries_per_sequence(D, Hq, H, bs, dtype):
 @pytest.mark.parametrize("D,Hq,H", [(128, 8, 2), (64, 6, 1), (128, 1, 1)])
 def test_prompt_chunks(queries, lens, D, Hq, H):
     _check_attention(gen(sum(queries)), lens, queries, Hq, H, D, 16, torch.bfloat16 if D == 128 else torch.float16)
+
+
+# With wide tables the same calls take the persistent kernel: its shares then hold less than a page, parts of items, several items.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,Hq,H,bs", [(128, 8, 1, 16), (64, 10, 2, 32), (128, 16, 1, 48), (64, 16, 1, 16), (128, 12, 6, 16)])
+def test_wide_tables_single_queries(D, Hq, H, bs, dtype):
+    _check_attention(gen(Hq), [0, 1, 15, 16, 17, 31, 33, 64, 100, 257, 1000, -3, 2], [1] * 13, Hq, H, D, bs, dtype, width=512)
+
+
+@pytest.mark.parametrize("lens", [[1], [0, 0, 0], [5003, 0, 0, 7], [16 * 2368 // 4], [16 * 2368 // 4 + 1, 1], [40] * 700, list(range(0, 1400, 3))])
+@pytest.mark.parametrize("D,Hq,H", [(128, 8, 1), (64, 12, 4)])
+def test_wide_tables_shares(lens, D, Hq, H):
+    """Fewer pages than warps, one more than evenly shared, more sequences than entries of the prefix, shares of many items."""
+    _check_attention(gen(len(lens)), lens, [1] * len(lens), Hq, H, D, 16, torch.float16, width=5000 // len(lens) + 1200)
+
+
+@pytest.mark.parametrize("D,Hq,H,bs", [(128, 8, 2, 16), (64, 5, 1, 32), (128, 16, 1, 16), (128, 3, 3, 32)])
+def test_wide_tables_several_queries(D, Hq, H, bs):
+    lens, queries = [40, 1, 300, 17, 0, 2, 64, 33, 700], [4, 1, 7, 0, 3, 5, 6, 2, 8]
+    _check_attention(gen(Hq), lens, queries, Hq, H, D, bs, torch.bfloat16, width=600)
+
+
+def test_negative_and_zero_scales():
+    for width in (0, 1300):
+        _check_attention(gen(5), [300, 40], [1, 1], 8, 2, 128, 16, torch.float16, sm_scale=-0.05, width=width)
+        _check_attention(gen(6), [300, 40], [1, 1], 8, 2, 128, 16, torch.bfloat16, sm_scale=0.0, width=width)
 
 
 def test_scores_of_any_size():

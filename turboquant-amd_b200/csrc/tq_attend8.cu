@@ -109,7 +109,13 @@ __device__ __forceinline__ void load_queries(Rows<D, NT>& w, const Attend8Params
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[c][i] = 0;
         }
-        float row_scale = p.scale_log2;
+        float row_scale = fabsf(p.scale_log2);
+        if (p.scale_log2 < 0.f) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[c][i] ^= 0x80008000u;
+        }
         if constexpr (BF16) {
             uint32_t most = 0;
 #pragma unroll
@@ -211,28 +217,31 @@ template <int D, int NT>
 __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], float2 scales, int page, uint32_t (&weights)[NT][2]) {
     const int g = (threadIdx.x & 31) >> 2;
     const float ev = static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127);
+    float c[NT][2];         // positive: the sign of sm_scale is in the query
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c[n][j] = w.scale[n][j] * scales.x;
+    if (page * kPageTokens + kPageTokens > w.min_limit) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                s[n][j] = page * kPageTokens + g + 8 * (j >> 1) >= w.limit[n][j & 1] ? -__uint_as_float(0x7f800000u) : s[n][j] * c[n][j & 1];
+            c[n][0] = c[n][1] = 1.f;
+        }
+    }
     bool over = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] *= w.scale[n][j & 1] * scales.x;
-    if (page * kPageTokens + kPageTokens > w.min_limit) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (page * kPageTokens + g + 8 * (j >> 1) >= w.limit[n][j & 1]) s[n][j] = -__uint_as_float(0x7f800000u);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) over |= fmaxf(s[n][j], s[n][j + 2]) > fminf(w.m[n][j], w.u[n][j] - ev) + kLazy;
+        for (int j = 0; j < 2; ++j) over |= fmaxf(s[n][j], s[n][j + 2]) * c[n][j] > fminf(w.m[n][j], w.u[n][j] - ev) + kLazy;
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float most = fmaxf(s[n][j], s[n][j + 2]);
+                float most = fmaxf(s[n][j], s[n][j + 2]) * c[n][j];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 const float m = fmaxf(w.m[n][j], most), u = fmaxf(w.u[n][j], most + ev);
@@ -252,8 +261,8 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
         float e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            w.l[n][j & 1] += ex2(s[n][j] - w.m[n][j & 1]);
-            e[j] = ex2(s[n][j] - (w.u[n][j & 1] - ev - kHeadroom));
+            w.l[n][j & 1] += ex2(fmaf(s[n][j], c[n][j & 1], -w.m[n][j & 1]));
+            e[j] = ex2(fmaf(s[n][j], c[n][j & 1], ev + kHeadroom - w.u[n][j & 1]));
         }
         weights[n][0] = movmatrix_trans(pack_half2(e[0], e[1]));      // tokens 2t, 2t + 1 of column g
         weights[n][1] = movmatrix_trans(pack_half2(e[2], e[3]));
@@ -268,7 +277,7 @@ __device__ __forceinline__ void page_products(Rows<D, NT>& w, const Page<D>& x, 
         return;
     }
     const int most = min(w.max_limit - first, kPageTokens), least = max(min(w.min_limit - first, kPageTokens), 0);
-    if (most == least || !has_nan<D>(x, least, lane)) {
+    if (most <= least || !has_nan<D>(x, least, lane)) {
         page_values<D, NT, true>(w.o, x, weights, most, lane);
         return;
     }
@@ -471,16 +480,27 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params 
     for (int i = 0; i < D / 32; ++i) store_out(p.out, at * D + lane + 32 * i, l == 0.f ? 0.f : o[i] / l, bf16 != 0);
 }
 
+}  // namespace
+}  // namespace tq
+
+#include "tq_attend8_stream.cuh"
+
+namespace tq {
+namespace {
+
 struct Attend8Plan {
+    bool stream;
     int nt, tiles, chunk_pages, chunks;
 };
 
+// Which kernel, and how it is cut.  The persistent one needs a page or two per warp of the GPU at least.
 Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
-    Attend8Plan a;
+    Attend8Plan a = {};
     const int64_t rows = static_cast<int64_t>(group) * max_queries;
     a.nt = rows <= 8 ? 1 : 2;
     a.tiles = static_cast<int>((rows + 8 * a.nt - 1) / (8 * a.nt));
     const int64_t items = seqs * kv_heads * a.tiles;
+    a.stream = items * max_pages >= 4736;
     int64_t want = (148 * 4 + items - 1) / items;                       // chunks per item that fill the GPU
     const int64_t most = (max_pages + 15) / 16;
     if (want > most) want = most;
@@ -492,15 +512,41 @@ Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries,
     return a;
 }
 
+int64_t attend8_workspace(const Attend8Plan& a, int64_t rows, int q_heads, int head_dim) {
+    if (a.stream)
+        return 4 * (head_dim == 64 ? (a.nt == 1 ? StreamSpace<64, 1>::kFloats : StreamSpace<64, 2>::kFloats)
+                                   : (a.nt == 1 ? StreamSpace<128, 1>::kFloats : StreamSpace<128, 2>::kFloats));
+    return a.chunks == 1 ? 0 : rows * q_heads * a.chunks * (head_dim + 2) * 4;
+}
+
+template <int D, int NT, bool BF16>
+cudaError_t launch_kernel(const Attend8Params& p, bool stream_kernel, cudaStream_t stream) {
+    if (!stream_kernel) {
+        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
+        cudaError_t err = launch_chained(attend8_kernel<D, NT, BF16>, grid, dim3(kWarps * 32), 0, stream, p);
+        if (err != cudaSuccess || p.chunks == 1) return err;
+        return launch_chained(attend8_merge_kernel<D>, dim3(static_cast<unsigned>(p.merge_blocks) * p.seqs), dim3(128), 0, stream, p, static_cast<int>(BF16));
+    }
+    auto kernel = attend8_stream_kernel<D, NT, BF16>;
+    // The opt-in shared-memory size is a per-device function attribute; set once per device.
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!configured[dev]) {
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamSmem<D, NT>::kBytes);
+        if (err != cudaSuccess) return err;
+        configured[dev] = true;
+    }
+    err = launch_chained(kernel, dim3(kMaxCtas), dim3(stream_warps(NT) * 32), StreamSmem<D, NT>::kBytes, stream, p);
+    if (err != cudaSuccess) return err;
+    return launch_chained(attend8_stream_merge_kernel<D, NT, BF16>, dim3(kMaxCtas - 1, NT), dim3(256), 0, stream, p);
+}
+
 template <int D>
-cudaError_t launch_attend8(const Attend8Params& p, int nt, bool bf16, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs)), block(kWarps * 32);
-    cudaError_t err;
-    if (nt == 1) err = bf16 ? launch_chained(attend8_kernel<D, 1, true>, grid, block, 0, stream, p) : launch_chained(attend8_kernel<D, 1, false>, grid, block, 0, stream, p);
-    else err = bf16 ? launch_chained(attend8_kernel<D, 2, true>, grid, block, 0, stream, p) : launch_chained(attend8_kernel<D, 2, false>, grid, block, 0, stream, p);
-    if (err != cudaSuccess || p.chunks == 1) return err;
-    const dim3 merge(static_cast<unsigned>(p.merge_blocks) * p.seqs);
-    return launch_chained(attend8_merge_kernel<D>, merge, dim3(128), 0, stream, p, static_cast<int>(bf16));
+cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, bool bf16, cudaStream_t stream) {
+    if (a.nt == 1) return bf16 ? launch_kernel<D, 1, true>(p, a.stream, stream) : launch_kernel<D, 1, false>(p, a.stream, stream);
+    return bf16 ? launch_kernel<D, 2, true>(p, a.stream, stream) : launch_kernel<D, 2, false>(p, a.stream, stream);
 }
 
 }  // namespace
@@ -514,7 +560,7 @@ extern "C" int64_t tq_attend8_workspace_bytes(int64_t num_rows, int num_seqs, in
     if (head_dim != 64 && head_dim != 128) return TQ_ERR_UNSUPPORTED;
     if (num_seqs == 0) return 0;
     const Attend8Plan a = attend8_plan(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
-    return a.chunks == 1 ? 0 : num_rows * num_q_heads * a.chunks * (head_dim + 2) * 4;
+    return attend8_workspace(a, num_rows, num_q_heads, head_dim);
 }
 
 extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const void* cache, int64_t num_blocks, int block_size,
@@ -542,7 +588,7 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     const int64_t merge_blocks = (static_cast<int64_t>(max_queries) * num_q_heads + 3) / 4;
     if (static_cast<double>(num_kv_heads) * a.tiles * a.chunks * num_seqs > INT32_MAX || static_cast<double>(merge_blocks) * num_seqs > INT32_MAX)
         return TQ_ERR_UNSUPPORTED;
-    const int64_t need = a.chunks == 1 ? 0 : num_rows * num_q_heads * a.chunks * (head_dim + 2) * 4;
+    const int64_t need = attend8_workspace(a, num_rows, num_q_heads, head_dim);
     if (need && (!workspace || workspace_bytes < need)) return TQ_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return TQ_ERR_ARG;
     Attend8Params p = {};
@@ -551,7 +597,7 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     p.scale_log2 = sm_scale * kLog2e; p.rows = static_cast<int>(num_rows); p.seqs = num_seqs; p.q_heads = num_q_heads; p.kv_heads = num_kv_heads;
     p.group = num_q_heads / num_kv_heads; p.pages_per_block = block_size / kPageTokens; p.max_pages = max_pages_per_seq; p.max_queries = max_queries;
     p.tiles = a.tiles; p.tile_rows = 8 * a.nt; p.merge_blocks = static_cast<int>(merge_blocks); p.chunk_pages = a.chunk_pages; p.chunks = a.chunks; p.zero_tail = zero_tail;
-    const cudaError_t err = head_dim == 64 ? launch_attend8<64>(p, a.nt, io_dtype == TQ_DTYPE_BF16, stream)
-                                           : launch_attend8<128>(p, a.nt, io_dtype == TQ_DTYPE_BF16, stream);
+    const cudaError_t err = head_dim == 64 ? launch_attend8<64>(p, a, io_dtype == TQ_DTYPE_BF16, stream)
+                                           : launch_attend8<128>(p, a, io_dtype == TQ_DTYPE_BF16, stream);
     return err == cudaSuccess ? TQ_OK : TQ_ERR_LAUNCH;
 }

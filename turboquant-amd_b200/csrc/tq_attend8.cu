@@ -461,10 +461,13 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params 
     if (r >= nq * p.q_heads) return;
     const int token = r / p.q_heads, head = r - token * p.q_heads, kvh = head / p.group, row = token * p.group + head - kvh * p.group;
     const int len = min(p.seq_lens[seq], p.max_pages * kPageTokens);
-    const int last = min(row / p.tile_rows * p.tile_rows + p.tile_rows - 1, nq * p.group - 1);
-    const int pages = pages_of_length(len - nq + last / p.group + 1);
-    const int chunks = (pages + p.chunk_pages - 1) / p.chunk_pages;
-    if (chunks <= 1) return;                         // written by its only chunk
+    int chunks = p.chunks;                              // prompt chunks: every part is written
+    if (p.chunk_pages) {
+        const int last = min(row / p.tile_rows * p.tile_rows + p.tile_rows - 1, nq * p.group - 1);
+        const int pages = pages_of_length(len - nq + last / p.group + 1);
+        chunks = (pages + p.chunk_pages - 1) / p.chunk_pages;
+        if (chunks <= 1) return;                     // written by its only chunk
+    }
     const int64_t at = static_cast<int64_t>(first_row + token) * p.q_heads + head;
     const float* part = p.partials + at * p.chunks * (D + 2);
     float m = kNothing;
@@ -484,23 +487,36 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params 
 }  // namespace tq
 
 #include "tq_attend8_stream.cuh"
+#include "tq_attend8_prompt.cuh"
 
 namespace tq {
 namespace {
 
+enum class Attend8Kind { kChunks, kStream, kPrompt };
+
 struct Attend8Plan {
-    bool stream;
+    Attend8Kind kind;
     int nt, tiles, chunk_pages, chunks;
 };
 
-// Which kernel, and how it is cut.  The persistent one needs a page or two per warp of the GPU at least.
+// Which kernel, and how it is cut.
 Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
     Attend8Plan a = {};
     const int64_t rows = static_cast<int64_t>(group) * max_queries;
+    if (rows > 32) {
+        a.kind = Attend8Kind::kPrompt;
+        a.tiles = static_cast<int>((rows + 2 * kTile - 1) / (2 * kTile));
+        const int64_t items = seqs * kv_heads * a.tiles, steps = (max_pages + 2 * kTilePages - 1) / (2 * kTilePages);
+        int64_t want = kMaxCtas / items;                                // parts per item, of two steps at least, that fill the GPU
+        if (want > steps) want = steps;
+        a.chunks = static_cast<int>(want < 1 ? 1 : want);
+        return a;
+    }
     a.nt = rows <= 8 ? 1 : 2;
     a.tiles = static_cast<int>((rows + 8 * a.nt - 1) / (8 * a.nt));
     const int64_t items = seqs * kv_heads * a.tiles;
-    a.stream = items * max_pages >= 4736;
+    // The persistent kernel needs a page or two per warp of the GPU at least.
+    a.kind = items * max_pages >= 4736 ? Attend8Kind::kStream : Attend8Kind::kChunks;
     int64_t want = (148 * 4 + items - 1) / items;                       // chunks per item that fill the GPU
     const int64_t most = (max_pages + 15) / 16;
     if (want > most) want = most;
@@ -513,31 +529,40 @@ Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries,
 }
 
 int64_t attend8_workspace(const Attend8Plan& a, int64_t rows, int q_heads, int head_dim) {
-    if (a.stream)
+    if (a.kind == Attend8Kind::kStream)
         return 4 * (head_dim == 64 ? (a.nt == 1 ? StreamSpace<64, 1>::kFloats : StreamSpace<64, 2>::kFloats)
                                    : (a.nt == 1 ? StreamSpace<128, 1>::kFloats : StreamSpace<128, 2>::kFloats));
     return a.chunks == 1 ? 0 : rows * q_heads * a.chunks * (head_dim + 2) * 4;
 }
 
-template <int D, int NT, bool BF16>
-cudaError_t launch_kernel(const Attend8Params& p, bool stream_kernel, cudaStream_t stream) {
-    if (!stream_kernel) {
-        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
-        cudaError_t err = launch_chained(attend8_kernel<D, NT, BF16>, grid, dim3(kWarps * 32), 0, stream, p);
-        if (err != cudaSuccess || p.chunks == 1) return err;
-        return launch_chained(attend8_merge_kernel<D>, dim3(static_cast<unsigned>(p.merge_blocks) * p.seqs), dim3(128), 0, stream, p, static_cast<int>(BF16));
-    }
-    auto kernel = attend8_stream_kernel<D, NT, BF16>;
-    // The opt-in shared-memory size is a per-device function attribute; set once per device.
-    static bool configured[64] = {};
+// The opt-in shared-memory size is a per-device function attribute; set once per device.
+template <typename Kernel>
+cudaError_t allow_shared_memory(Kernel kernel, int bytes, bool (&configured)[64]) {
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!configured[dev]) {
-        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamSmem<D, NT>::kBytes);
-        if (err != cudaSuccess) return err;
-        configured[dev] = true;
+    if (configured[dev]) return cudaSuccess;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    configured[dev] = err == cudaSuccess;
+    return err;
+}
+
+template <int D>
+cudaError_t launch_merge(const Attend8Params& p, bool bf16, cudaStream_t stream) {
+    return launch_chained(attend8_merge_kernel<D>, dim3(static_cast<unsigned>(p.merge_blocks) * p.seqs), dim3(128), 0, stream, p, static_cast<int>(bf16));
+}
+
+template <int D, int NT, bool BF16>
+cudaError_t launch_rows(const Attend8Params& p, bool persistent, cudaStream_t stream) {
+    if (!persistent) {
+        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
+        const cudaError_t err = launch_chained(attend8_kernel<D, NT, BF16>, grid, dim3(kWarps * 32), 0, stream, p);
+        return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, BF16, stream);
     }
+    static bool configured[64] = {};
+    auto kernel = attend8_stream_kernel<D, NT, BF16>;
+    cudaError_t err = allow_shared_memory(kernel, StreamSmem<D, NT>::kBytes, configured);
+    if (err != cudaSuccess) return err;
     err = launch_chained(kernel, dim3(kMaxCtas), dim3(stream_warps(NT) * 32), StreamSmem<D, NT>::kBytes, stream, p);
     if (err != cudaSuccess) return err;
     return launch_chained(attend8_stream_merge_kernel<D, NT, BF16>, dim3(kMaxCtas - 1, NT), dim3(256), 0, stream, p);
@@ -545,8 +570,17 @@ cudaError_t launch_kernel(const Attend8Params& p, bool stream_kernel, cudaStream
 
 template <int D>
 cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, bool bf16, cudaStream_t stream) {
-    if (a.nt == 1) return bf16 ? launch_kernel<D, 1, true>(p, a.stream, stream) : launch_kernel<D, 1, false>(p, a.stream, stream);
-    return bf16 ? launch_kernel<D, 2, true>(p, a.stream, stream) : launch_kernel<D, 2, false>(p, a.stream, stream);
+    if (a.kind == Attend8Kind::kPrompt) {
+        static bool configured[64] = {};
+        cudaError_t err = allow_shared_memory(attend8_prompt_kernel<D>, PromptSmem<D>::kBytes, configured);
+        if (err != cudaSuccess) return err;
+        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
+        err = launch_chained(attend8_prompt_kernel<D>, grid, dim3(kPromptThreads), PromptSmem<D>::kBytes, stream, p, static_cast<int>(bf16));
+        return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, bf16, stream);
+    }
+    const bool persistent = a.kind == Attend8Kind::kStream;
+    if (a.nt == 1) return bf16 ? launch_rows<D, 1, true>(p, persistent, stream) : launch_rows<D, 1, false>(p, persistent, stream);
+    return bf16 ? launch_rows<D, 2, true>(p, persistent, stream) : launch_rows<D, 2, false>(p, persistent, stream);
 }
 
 }  // namespace
@@ -574,7 +608,7 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
         return TQ_ERR_ARG;
     if ((io_dtype != TQ_DTYPE_F16 && io_dtype != TQ_DTYPE_BF16) || (head_dim != 64 && head_dim != 128)) return TQ_ERR_UNSUPPORTED;
     if (block_size < kPageTokens || block_size % kPageTokens || num_blocks > INT32_MAX || num_rows > INT32_MAX) return TQ_ERR_UNSUPPORTED;
-    if (max_pages_per_seq > (1 << 27) - 1 || static_cast<int64_t>(max_queries) * num_q_heads > (1 << 30)) return TQ_ERR_UNSUPPORTED;
+    if (max_pages_per_seq > (1 << 26) || static_cast<int64_t>(max_queries) * num_q_heads > (1 << 30)) return TQ_ERR_UNSUPPORTED;
     if (num_rows == 0) return TQ_OK;
     if (num_seqs == 0) {
         if (!zero_tail) return TQ_OK;

@@ -3,19 +3,23 @@
 // A CTA takes 256 query rows (two tiles of 128; rows are token-major, the heads of a group side by side) of one sequence and KV head
 // and walks over the keys, 128 tokens at a time:
 //
-//   converter warps 8-11  read the codes of a tile's 8 pages (16 bytes a lane), bring pages to one power-of-two scale while they
-//                         turn them into fp16 - exact, e4m3 has 4 significant bits - and write both operands into shared memory:
-//                         K as K-major B operand, V as MN-major one.  An earlier form of the product in e4m3 itself would
-//                         need the queries and weights as sums of two or three e4m3 terms, which costs more than the conversion
+//   planner warp 13       looks up the blocks and scales of the tiles to come and has their codes copied into shared memory (bulk copies,
+//                         2 KB of a page each)
+//   converter warps       8, 9: keys, 10, 11: values: codes to fp16 - exact, whatever the scale - as operands in shared memory, K K-major,
+//                         V MN-major.  (A product in e4m3 itself would need queries and weights as sums of two or three e4m3 terms,
+//                         which costs more)
 //   MMA warp 12           one thread: S_q = Q_q K^T (shared x shared), O_q += P_q V (tensor memory x shared), q = 0, 1
 //   softmax warps 0-3, 4-7  thread = query row of tile 0 / 1: maximum, weights in fp16 back into the columns of S, sums
 //
 // The two tiles take turns: while one's weights are computed, the tensor cores work on the other's products.  The references of the softmax
 // are raised only when a score passes them by 2^8, so that O in tensor memory is rarely rescaled.  Bound: the exponentials (16 a cycle
 // and SM, 2048 cycles a tile pair) next to the products (2048 cycles); conversion and bookkeeping share the issue slots with them.
+// Four roles run different code at the same time, and what they repeat has to fit the instruction cache: with everything unrolled (28 KB of
+// instructions a step) it missed in 28 % of the cases, the next level was at 77 % of its rate, and a step took 7000 cycles.
+// So loops stay loops here, and the codes go through shared memory instead of registers.
 //
-// Scales of V that are far apart: fp16 holds codes exactly for pages within 2^15 of the tile's largest scale.  A tile with more is walked
-// over several times, each time with the pages of one range (others masked), so that no page's values lose bits to another's.
+// The pages' scales enter with the weights, as two numbers for each 16 columns of the scores: weight = 2^(s c_page + shift_page), so that
+// fp16 weights use their range whatever the scales are (page_weights in tq_attend8.cu has the same two references m and u).
 // A NaN in V counts as zero in the product; its dim and token are noted, and rows that see the token become NaN in that dim at the end.
 //
 // All waits are bounded; one that gives up sets TQ_STATUS_TIMEOUT, every role leaves its loop and the tensor memory is freed.
@@ -24,33 +28,37 @@
 namespace tq {
 namespace {
 
-constexpr int kPromptThreads = 13 * 32;
+constexpr int kPromptThreads = 14 * 32;
 constexpr int kTile = 128;                      // query rows of a tile, and tokens of a step
 constexpr int kTilePages = kTile / kPageTokens;
-constexpr int kDescs = 4;
+constexpr int kPlans = 8;
 
-struct StepDesc {
-    int token0, mask, last, v_exp;
-    float k_scale;
-    int pad[3];
+// The scales of a tile's pages: of K as it is, of V as the power of two.
+struct StepPlan {
+    float k_scale[kTilePages], v_exp[kTilePages];
+    int token0, last, pad[2];
 };
 
 template <int D>
 struct PromptSmem {
     static constexpr int kOperand = kTile * D * 2;                       // bytes of a tile of queries, keys or values
     static constexpr int kBars = 0;
-    static constexpr int kTmemSlot = 128;
-    static constexpr int kFlags = 132;                                   // failed, NaN seen
-    static constexpr int kDesc = 144;
-    static constexpr int kNan = kDesc + kDescs * 32;                     // [D] first token with a NaN in this dim of V
-    static constexpr int kQ = 1024;                                      // [2]
+    static constexpr int kTmemSlot = 256;
+    static constexpr int kFlags = 260;                                   // failed, NaN seen
+    static constexpr int kPlan = 272;
+    static constexpr int kNan = kPlan + kPlans * sizeof(StepPlan);       // [D] first token with a NaN in this dim of V
+    static constexpr int kQ = 2048;                                      // [2]
     static constexpr int kK = kQ + 2 * kOperand;                         // [2]
     static constexpr int kV = kK + 2 * kOperand;                         // [2]
-    static constexpr int kBytes = kV + 2 * kOperand;
-    static_assert(kNan + D * 4 <= kQ, "shared memory map");
+    static constexpr int kRawK = kV + 2 * kOperand;                      // codes of a tile's keys, values
+    static constexpr int kRawV = kRawK + kTile * D;
+    static constexpr int kBytes = kRawV + kTile * D;
+    static_assert(kNan + D * 4 <= kQ && kBytes <= 227 * 1024, "shared memory map");
 };
 
-enum PromptBar { kbKFull = 0, kbKEmpty = 2, kbVFull = 4, kbVEmpty = 6, kbSFull = 8, kbPFull = 10, kbPvDone = 12 };
+enum PromptBar { kbKFull = 0, kbKEmpty = 2, kbVFull = 4, kbVEmpty = 6, kbSFull = 8, kbPFull = 10, kbPvDone = 12, kbRawKFull = 14, kbRawKEmpty = 15, kbRawVFull = 16, kbRawVEmpty = 17,
+                 kbPlanEmpty = 18, kbBars = 18 + kPlans };
+static_assert(kbBars * 8 <= 256, "barriers");
 
 __device__ __forceinline__ void prompt_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -88,18 +96,34 @@ __device__ __forceinline__ void prompt_ld32(uint32_t at, uint32_t (&r)[32]) {
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(at) : "memory");
 }
-__device__ __forceinline__ void prompt_st32(uint32_t at, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+__device__ __forceinline__ void prompt_ld16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at) : "memory");
 }
 __device__ __forceinline__ void prompt_st16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+
+// two fp32 in one register pair
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 __device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -113,9 +137,8 @@ struct PromptJob {
     int token_a, token_b;                       // tokens that this CTA walks over
 };
 
-// 16 codes times 2^d, as fp16, into two 16-byte pieces.
-template <bool VALUES>
-__device__ __forceinline__ void convert16(uint4 codes, uint32_t factor, bool plain, uint32_t at, uint32_t step) {
+// 16 codes as fp16 into two 16-byte pieces.
+__device__ __forceinline__ void convert16(uint4 codes, uint32_t at, uint32_t step) {
     const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
     uint32_t h[8];
 #pragma unroll
@@ -123,205 +146,211 @@ __device__ __forceinline__ void convert16(uint4 codes, uint32_t factor, bool pla
         h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
         h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
     }
-    if (!plain) {
-        const __half2 f = *reinterpret_cast<const __half2*>(&factor);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), f);
-            h[i] = *reinterpret_cast<const uint32_t*>(&x);
-        }
-    }
     sts16(at, h[0], h[1], h[2], h[3]);
     sts16(at + step, h[4], h[5], h[6], h[7]);
 }
 
-// 2^d as half2: exact down to 2^-24, zero below
-__device__ __forceinline__ uint32_t half2_power(int d) {
-    const uint32_t h = d >= -14 ? static_cast<uint32_t>(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
-    return h | h << 16;
-}
-
+// Lane i < 8 looks at page i of a tile, and has its keys copied, lane 8 + i its values.
 template <int D>
-__device__ void prompt_convert(const Attend8Params& p, const PromptJob& job, int seq, uint8_t* smem, uint64_t* bars, volatile int* flags) {
+__device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int seq, uint8_t* smem, uint64_t* bars, volatile int* flags) {
     using Smem = PromptSmem<D>;
-    constexpr int kLoads = D / 32;               // 16-byte pieces of a lane and page
-    constexpr uint32_t kColumn = 2048;           // K: bytes between 8-dim columns.  V: between groups of 8 tokens it is D * 16
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - 8;
-    const uint32_t base = smem_u32(smem);
+    constexpr uint32_t kPart = kPageTokens * D;
+    const int lane = threadIdx.x & 31, mine = lane & 7;
     const int32_t* table = p.tables + seq * p.table_stride;
     const int pages = pages_of_length(job.token_b);
-    const int tok = lane & 15, half = lane >> 4;
-    int* first_nan = reinterpret_cast<int*>(smem + Smem::kNan);
-    StepDesc* descs = reinterpret_cast<StepDesc*>(smem + Smem::kDesc);
+    StepPlan* plans = reinterpret_cast<StepPlan*>(smem + Smem::kPlan);
     bool bad = false;
-
-    // Lane i < 8 knows page i of a tile: its block (asked for two tiles ahead) and its scales (one tile ahead, with the codes).
     auto ask_block = [&](int token0) {
-        const int page = token0 / kPageTokens + (lane & 7);
-        int block = -1;
-        if (page < pages) {
-            block = __ldg(table + page / p.pages_per_block);
-            if (block < 0 || block >= p.num_blocks) {
-                bad = true;
-                block = block < 0 ? 0 : static_cast<int>(p.num_blocks - 1);
-            }
-        }
-        return block;
+        const int page = token0 / kPageTokens + mine;
+        return page < pages ? __ldg(table + page / p.pages_per_block) : 0;
     };
-    uint4 k[2][kLoads], v[2][kLoads];
-    float2 scales = make_float2(0.f, 0.f);
-    auto page_at = [&](int token0, int i, int block) { return page_address<D>(p, token0 / kPageTokens + i, block, job.kvh); };
-    auto ask_scales = [&](int token0, int block) {
-        scales = block >= 0 ? __ldg(reinterpret_cast<const float2*>(page_at(token0, lane & 7, block) + cache8_scale_off(D))) : make_float2(0.f, 0.f);
-    };
-    auto ask_codes = [&](int token0, int block, bool values, uint4 (&x)[2][kLoads]) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int b = __shfl_sync(0xffffffffu, block, 2 * warp + i);
-            const uint8_t* at = b >= 0 ? page_at(token0, 2 * warp + i, b) + (values ? kPageTokens * D : 0) + tok * D + half * 16 : nullptr;
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j) x[i][j] = b >= 0 ? __ldg(reinterpret_cast<const uint4*>(at + j * 32)) : make_uint4(0, 0, 0, 0);
+    int block = ask_block(job.token_a), step = 0;
+    for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
+        const int page = token0 / kPageTokens + mine, count = min(pages - token0 / kPageTokens, kTilePages);
+        const bool here = mine < count;
+        if (here && (block < 0 || block >= p.num_blocks)) {
+            bad = true;
+            block = block < 0 ? 0 : static_cast<int>(p.num_blocks - 1);
         }
-    };
-    int block = ask_block(job.token_a);
-    ask_scales(job.token_a, block);
-    ask_codes(job.token_a, block, false, k);
-    ask_codes(job.token_a, block, true, v);
-    block = ask_block(job.token_a + kTile);
-    int step = 0;
-    for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile) {
-        const bool last_tile = token0 + kTile >= job.token_b;
-        const int ke = exponent_of_scale_bits(__float_as_uint(scales.x)), ve = exponent_of_scale_bits(__float_as_uint(scales.y));
-        const bool here = token0 / kPageTokens + (lane & 7) < pages;
-        const int k_ref = __reduce_max_sync(0xffffffffu, here ? ke : kMinExponent);
-        uint32_t todo = 0xffu;                                              // pages that are still to come
-        while (todo) {
-            // The pages within 2^15 of the largest scale left; pages whose values are all zeros go with any.
-            const bool open = todo >> (lane & 7) & 1, counts = here && ve > kMinExponent;
-            const int v_ref = __reduce_max_sync(0xffffffffu, open && counts ? ve : kMinExponent);
-            const uint32_t group = __ballot_sync(0xffffffffu, open && (!counts || ve >= v_ref - 15)) & 0xffu;
-            todo &= ~group;
-            const bool last = last_tile && !todo;
-            const int s = step & 1;
-            const uint32_t turn = (step >> 1 & 1) ^ 1;
-            if (!mbar_wait_bounded(bars + kbKEmpty + s, turn)) flags[0] = 1;
-            if (warp == 0 && lane == 0) {
-                StepDesc& d = descs[step % kDescs];
-                d.token0 = token0;
-                d.mask = static_cast<int>(group);
-                d.last = last;
-                d.v_exp = v_ref;
-                d.k_scale = exp2_int(k_ref);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int page = 2 * warp + i;
-                const int d = max(__shfl_sync(0xffffffffu, ke, page) - k_ref, -126);
-                const uint32_t f = half2_power(d);
-                const uint32_t to = base + Smem::kK + s * Smem::kOperand + (page * kPageTokens + tok) * 16 + half * 2 * kColumn;
-#pragma unroll
-                for (int j = 0; j < kLoads; ++j) convert16<false>(k[i][j], f, d == 0, to + j * 4 * kColumn, kColumn);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) prompt_arrive(bars + kbKFull + s);
-            if (!todo && !last) ask_codes(token0 + kTile, block, false, k);  // the next tile's, behind this one's last use
-
-            if (!mbar_wait_bounded(bars + kbVEmpty + s, turn)) flags[0] = 1;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int page = 2 * warp + i;
-                const int d = max(min(__shfl_sync(0xffffffffu, ve, page) - v_ref, 0), -126);
-                const bool in = group >> page & 1;
-                const uint32_t f = in ? half2_power(d) : 0u;
-                const int token = page * kPageTokens + tok;
-                const uint32_t to = base + Smem::kV + s * Smem::kOperand + (token >> 3) * (D * 16) + (token & 7) * 16 + half * 256;
-#pragma unroll
-                for (int j = 0; j < kLoads; ++j) {
-                    uint4 x = v[i][j];
-                    uint32_t nan[4] = {x.x, x.y, x.z, x.w}, any = 0;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        nan[w] = ((nan[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                        any |= nan[w];
-                    }
-                    if (any) {
-                        flags[1] = 1;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w)
-#pragma unroll
-                            for (int b = 0; b < 4; ++b)
-                                if (nan[w] >> (8 * b + 7) & 1) atomicMin(first_nan + (2 * j + half) * 16 + 4 * w + b, token0 + token);
-                        x.x &= ~((nan[0] >> 7) * 0xffu);
-                        x.y &= ~((nan[1] >> 7) * 0xffu);
-                        x.z &= ~((nan[2] >> 7) * 0xffu);
-                        x.w &= ~((nan[3] >> 7) * 0xffu);
-                    }
-                    convert16<true>(x, f, in && d == 0, to + j * 512, 128);
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) prompt_arrive(bars + kbVFull + s);
-            if (!todo && !last) {
-                ask_codes(token0 + kTile, block, true, v);
-                ask_scales(token0 + kTile, block);
-                block = ask_block(token0 + 2 * kTile);
-            }
-            ++step;
-            if (flags[0]) todo = 0;
-        }
+        const uint8_t* at = here ? page_address<D>(p, page, block, job.kvh) : nullptr;
+        block = ask_block(token0 + kTile);
+        const float2 scales = here ? __ldg(reinterpret_cast<const float2*>(at + cache8_scale_off(D))) : make_float2(0.f, 0.f);
+        // Pages that are not there keep the codes of another tile: their columns are masked, and finite values times zero are zero.
+        const uint32_t turn = (step & 1) ^ 1;
+        if (!mbar_wait_bounded(bars + kbRawKEmpty, turn)) flags[0] = 1;
         if (flags[0]) break;
+        if (lane == 0) mbar_expect_tx(bars + kbRawKFull, count * kPart);
+        __syncwarp();
+        if (here && lane < 8) bulk_g2s(smem + Smem::kRawK + mine * kPart, at, kPart, bars + kbRawKFull);
+        const int slot = step % kPlans;
+        if (!mbar_wait_bounded(bars + kbPlanEmpty + slot, (step / kPlans & 1) ^ 1)) flags[0] = 1;
+        if (!mbar_wait_bounded(bars + kbRawVEmpty, turn)) flags[0] = 1;
+        if (flags[0]) break;
+        StepPlan& plan = plans[slot];
+        if (lane < kTilePages) {
+            plan.k_scale[mine] = scales.x;
+            plan.v_exp[mine] = static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127);
+        }
+        if (lane == 0) {
+            plan.token0 = token0;
+            plan.last = token0 + kTile >= job.token_b;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(bars + kbRawVFull, count * kPart);       // tells of the plan, too: its writes come before
+        __syncwarp();
+        if (here && lane >= 8 && lane < 16) bulk_g2s(smem + Smem::kRawV + mine * kPart, at + kPart, kPart, bars + kbRawVFull);
     }
     if (bad && p.status) atomicOr(p.status, TQ_STATUS_BAD_BLOCK);
 }
 
+// A warp converts 4 pages of a tile, keys or values.
+template <int D, bool VALUES>
+__device__ void prompt_convert(const PromptJob& job, uint8_t* smem, uint64_t* bars, volatile int* flags) {
+    using Smem = PromptSmem<D>;
+    constexpr int kLoads = D / 32, kPages = kTilePages / 2;                 // 16-byte pieces of a lane and page
+    // K: 16 bytes (8 dims) of 128 tokens side by side.  V: of 8 tokens, then the next 8 dims, then the next 8 tokens.
+    constexpr uint32_t kColumn = VALUES ? 128 : 2048;
+    constexpr int kFull = VALUES ? kbVFull : kbKFull, kEmpty = VALUES ? kbVEmpty : kbKEmpty;
+    constexpr int kRawFull = VALUES ? kbRawVFull : kbRawKFull, kRawEmpty = VALUES ? kbRawVEmpty : kbRawKEmpty;
+    const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5 & 1) * kPages;
+    // A lane turns pieces (token, 2 j + half); the tokens of 8 lanes start on different banks where it stores, and where it loads the
+    // pieces of odd tokens are taken in another order
+    const int tok = lane & 15, half = lane >> 4;
+    const uint32_t base = smem_u32(smem), operand = base + (VALUES ? Smem::kV : Smem::kK), raw = base + (VALUES ? Smem::kRawV : Smem::kRawK);
+    int* first_nan = reinterpret_cast<int*>(smem + Smem::kNan);
+    int step = 0;
+    for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
+        const int s = step & 1;
+        if (!mbar_wait_bounded(bars + kRawFull, step & 1)) flags[0] = 1;
+        if (!mbar_wait_bounded(bars + kEmpty + s, (step >> 1 & 1) ^ 1)) flags[0] = 1;
+        if (flags[0]) return;
+#pragma unroll 1
+        for (int i = 0; i < kPages; ++i) {
+            const int token = (first + i) * kPageTokens + tok;
+            const uint32_t to = operand + s * Smem::kOperand + (VALUES ? (token >> 3) * (D * 16) + (token & 7) * 16 : token * 16);
+            uint4 x[kLoads];
+            uint32_t nan = 0;                                               // bit 7 of a byte: a code is 0x7f or 0xff
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) x[j] = lds16(raw + token * D + ((2 * j + half) ^ (tok & (2 * kLoads - 1))) * 16);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                if (VALUES)
+                    nan |= ((x[j].x & 0x7f7f7f7fu) + 0x01010101u) | ((x[j].y & 0x7f7f7f7fu) + 0x01010101u) |
+                           ((x[j].z & 0x7f7f7f7fu) + 0x01010101u) | ((x[j].w & 0x7f7f7f7fu) + 0x01010101u);
+                convert16(x[j], to + ((2 * j + half) ^ (tok & (2 * kLoads - 1))) * 2 * kColumn, kColumn);
+            }
+            if (VALUES && (nan & 0x80808080u)) {
+                // rare: this lane's pieces once more, from where they were put
+                flags[1] = 1;
+                asm volatile("" ::: "memory");
+#pragma unroll 1
+                for (int j = 0; j < kLoads * 16; ++j) {
+                    const int dim = ((2 * (j >> 4) + half) ^ (tok & (2 * kLoads - 1))) * 16 + (j & 15);
+                    uint16_t* at = reinterpret_cast<uint16_t*>(smem + (to - base) + (dim >> 3) * 128 + (dim & 7) * 2);
+                    if ((*at & 0x7fffu) > 0x7c00u) {
+                        *at = 0;
+                        atomicMin(first_nan + dim, token0 + token);
+                    }
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            prompt_arrive(bars + kRawEmpty);
+            prompt_arrive(bars + kFull + s);
+        }
+    }
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+// The whole warp walks through the steps, so that addresses and descriptors stay in uniform registers, and one lane issues.  (With a
+// single lane walking, the eight products of an operand took 1200 cycles to issue; they take 512 to run.)  All 512 columns
+// are this CTA's, so that they begin at address 0.
 template <int D>
-__device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* bars, volatile int* flags, uint32_t tmem) {
+__device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* bars, volatile int* flags) {
     using Smem = PromptSmem<D>;
     constexpr uint32_t kScores = prompt_idesc(kTile, 0), kOut = prompt_idesc(D, 1);
     const uint32_t base = smem_u32(smem);
-    const StepDesc* descs = reinterpret_cast<const StepDesc*>(smem + Smem::kDesc);
-    auto scores = [&](int q, int s) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-            prompt_mma_ss(tmem + q * kTile, prompt_desc(base + Smem::kQ + q * Smem::kOperand + i * 4096, 2048, 128),
-                          prompt_desc(base + Smem::kK + s * Smem::kOperand + i * 4096, 2048, 128), kScores, i ? 1u : 0u);
-        prompt_commit(bars + kbSFull + q);
-    };
+    const int steps = __shfl_sync(0xffffffffu, (job.token_b - job.token_a + kTile - 1) / kTile, 0);
+    const bool both = __shfl_sync(0xffffffffu, job.tiles, 0) == 2;
     auto wait = [&](int bar, uint32_t parity) {
         if (!mbar_wait_bounded(bars + bar, parity)) flags[0] = 1;
         return flags[0] == 0;
     };
+    const uint64_t queries = prompt_desc(base + Smem::kQ, 2048, 128), keys = prompt_desc(base + Smem::kK, 2048, 128),
+                   values = prompt_desc(base + Smem::kV, D * 16, 128);
+    auto scores = [&](int q, int s) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            prompt_mma_ss(q * kTile, queries + (q * Smem::kOperand + i * 4096) / 16, keys + (s * Smem::kOperand + i * 4096) / 16, kScores, i ? 1u : 0u);
+        prompt_commit(bars + kbSFull + q);
+    };
+    auto products = [&](int q, int s, uint32_t accumulate) {
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+            prompt_mma_ts(2 * kTile + q * kTile, q * kTile + i * 8, values + (s * Smem::kOperand + i * 2 * (D * 16)) / 16, kOut, i ? 1u : accumulate);
+        prompt_commit(bars + kbPvDone + q);
+    };
     if (!wait(kbKFull, 0)) return;
     prompt_fence_after();
-    for (int q = 0; q < job.tiles; ++q) scores(q, 0);
-    prompt_commit(bars + kbKEmpty);
-    for (int step = 0;; ++step) {
-        const int s = step & 1;
-        const bool last = *const_cast<const volatile int*>(&descs[step % kDescs].last);
+    if (elect_one()) {
+        scores(0, 0);
+        if (both) scores(1, 0);
+        prompt_commit(bars + kbKEmpty);
+    }
+    __syncwarp();
+    for (int step = 0; step < steps; ++step) {
+        const int s = step & 1, n = s ^ 1;
+        const bool more = step + 1 < steps;
         if (!wait(kbVFull + s, step >> 1 & 1)) return;
-        for (int q = 0; q < job.tiles; ++q) {
-            if (!wait(kbPFull + q, step & 1)) return;
-            prompt_fence_after();
-#pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-                prompt_mma_ts(tmem + 2 * kTile + q * kTile, tmem + q * kTile + i * 8,
-                              prompt_desc(base + Smem::kV + s * Smem::kOperand + i * 2 * (D * 16), D * 16, 128), kOut, step || i ? 1u : 0u);
-            prompt_commit(bars + kbPvDone + q);
-            if (q == job.tiles - 1) prompt_commit(bars + kbVEmpty + s);
-            if (!last) {
-                const int n = (step + 1) & 1;
-                if (q == 0) {
-                    if (!wait(kbKFull + n, (step + 1) >> 1 & 1)) return;
-                    prompt_fence_after();
-                }
-                scores(q, n);
-                if (q == job.tiles - 1) prompt_commit(bars + kbKEmpty + n);
+        if (!wait(kbPFull, step & 1)) return;
+        prompt_fence_after();
+        if (elect_one()) {
+            products(0, s, step ? 1u : 0u);
+            if (!both) {
+                prompt_commit(bars + kbVEmpty + s);
+                prompt_commit(bars + kbPlanEmpty + step % kPlans);
             }
         }
-        if (last) break;
+        __syncwarp();
+        if (more) {
+            if (!wait(kbKFull + n, (step + 1) >> 1 & 1)) return;
+            prompt_fence_after();
+            if (elect_one()) {
+                scores(0, n);
+                if (!both) prompt_commit(bars + kbKEmpty + n);
+            }
+            __syncwarp();
+        }
+        if (!both) continue;
+        if (!wait(kbPFull + 1, step & 1)) return;
+        prompt_fence_after();
+        if (elect_one()) {
+            products(1, s, step ? 1u : 0u);
+            prompt_commit(bars + kbVEmpty + s);
+            prompt_commit(bars + kbPlanEmpty + step % kPlans);              // the softmax warps are done with it, too
+            if (more) {
+                scores(1, n);
+                prompt_commit(bars + kbKEmpty + n);
+            }
+        }
+        __syncwarp();
     }
+}
+
+constexpr float kTiny = 1e-38f;             // factors of scores are never zero: times -inf that would be NaN
+
+// Columns from `visible` on see nothing.
+__device__ __forceinline__ void hide(uint32_t* x, int visible) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (i >= visible) x[i] = 0xff800000u;
 }
 
 template <int D>
@@ -334,95 +363,105 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
     const int warp_limit = __reduce_min_sync(0xffffffffu, limit);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + q * kTile, o_at = tmem + lanes + 2 * kTile + q * kTile;
-    const StepDesc* descs = reinterpret_cast<const StepDesc*>(smem + Smem::kDesc);
+    const StepPlan* plans = reinterpret_cast<const StepPlan*>(smem + Smem::kPlan);
     float m = kNothing, u = kNothing, l = 0.f;
     bool ok = true;
-    if (job.token_a < job.token_b) {
-        for (int step = 0;; ++step) {
-            if (!mbar_wait_bounded(bars + kbSFull + q, step & 1)) flags[0] = 1;
-            if (flags[0]) {
-                ok = false;
-                break;
-            }
-            prompt_fence_after();
-            const StepDesc d = descs[step % kDescs];
-            const float c = fmaxf(row_scale * d.k_scale, 1e-38f), ev = static_cast<float>(d.v_exp);
-            const bool masked = d.mask != 0xff || d.token0 + kTile > warp_limit;
-            const int visible = limit - d.token0;
-            float most = -__uint_as_float(0x7f800000u);
+    int step = 0;
+    for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
+        // the plan was written before the codes of V were asked for
+        if (!mbar_wait_bounded(bars + kbSFull + q, step & 1)) flags[0] = 1;
+        if (!mbar_wait_bounded(bars + kbVFull + (step & 1), step >> 1 & 1)) flags[0] = 1;
+        if (flags[0]) {
+            ok = false;
+            break;
+        }
+        prompt_fence_after();
+        const StepPlan& plan = plans[step % kPlans];
+        const bool masked = token0 + kTile > warp_limit;
+        const int visible = limit - token0;
+        float most = kNothing, most_v = kNothing;
+#pragma unroll 1
+        for (int h = 0; h < 4; h += 2) {
+            uint32_t x[2][32];
+            prompt_ld32(s_at + 32 * h, x[0]);
+            prompt_ld32(s_at + 32 * h + 32, x[1]);
+            prompt_wait_ld();
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                uint32_t x[32];
-                prompt_ld32(s_at + 32 * h, x);
-                prompt_wait_ld();
-                if (masked) {
+            for (int g = 0; g < 4; ++g) {
+                uint32_t* of = x[g >> 1] + 16 * (g & 1);
+                if (masked) hide(of, visible - 32 * h - 16 * g);
+                float a = __uint_as_float(of[0]);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * h + i >= visible || !(d.mask >> (2 * h + (i >> 4)) & 1)) x[i] = 0xff800000u;
-                }
-                float a = most, b = most;
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    a = fmaxf(fmaxf(a, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
-                    b = fmaxf(fmaxf(b, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
-                }
-                most = fmaxf(a, b);
-            }
-            most *= c;
-            if (__any_sync(0xffffffffu, most > fminf(m, u - ev) + kLazy)) {
-                const float m1 = fmaxf(m, most), u1 = fmaxf(u, most + ev);
-                l *= ex2(m - m1);
-                const float down = ex2(u - u1);
-                m = m1;
-                u = u1;
-                if (step) {
-                    // O is whole when the product of the step before is done
-                    if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
-                    prompt_fence_after();
-#pragma unroll
-                    for (int h = 0; h < D / 32; ++h) {
-                        uint32_t x[32];
-                        prompt_ld32(o_at + 32 * h, x);
-                        prompt_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * down);
-                        prompt_st32(o_at + 32 * h, x);
-                    }
-                }
-            }
-            const float shift = ev + kHeadroom - u;
-            float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                uint32_t x[32], w[16];
-                prompt_ld32(s_at + 32 * h, x);
-                prompt_wait_ld();
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * h + i >= visible || !(d.mask >> (2 * h + (i >> 4)) & 1)) x[i] = 0xff800000u;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float a = ex2(fmaf(__uint_as_float(x[2 * i]), c, shift)), b = ex2(fmaf(__uint_as_float(x[2 * i + 1]), c, shift));
-                    sum0 += a;
-                    sum1 += b;
-                    w[i] = pack_half2(a, b);
-                }
-                prompt_st16(s_at + 16 * h, w);
-            }
-            l = fmaf(sum0 + sum1, ex2(u - ev - kHeadroom - m), l);
-            prompt_wait_st();
-            prompt_fence_before();
-            __syncwarp();
-            if (lane == 0) prompt_arrive(bars + kbPFull + q);
-            if (d.last) {
-                if (!mbar_wait_bounded(bars + kbPvDone + q, step & 1)) flags[0] = 1;
-                ok = flags[0] == 0;
-                prompt_fence_after();
-                break;
+                for (int i = 1; i < 15; i += 2) a = fmaxf(fmaxf(a, __uint_as_float(of[i])), __uint_as_float(of[i + 1]));
+                a = fmaxf(a, __uint_as_float(of[15])) * fmaxf(row_scale * plan.k_scale[2 * h + g], kTiny);
+                most = fmaxf(most, a);
+                most_v = fmaxf(most_v, a + plan.v_exp[2 * h + g]);
             }
         }
+        if (__any_sync(0xffffffffu, most > m + kLazy || most_v > u + kLazy)) {
+            const float m1 = fmaxf(m, most), u1 = fmaxf(u, most_v);
+            l *= ex2(m - m1);
+            const float down = ex2(u - u1);
+            m = m1;
+            u = u1;
+            if (step) {
+                // O is whole when the product of the step before is done
+                if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
+                prompt_fence_after();
+#pragma unroll 1
+                for (int h = 0; h < D / 16; ++h) {
+                    uint32_t o[16];
+                    prompt_ld16(o_at + 16 * h, o);
+                    prompt_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
+                    prompt_st16(o_at + 16 * h, o);
+                }
+            }
+        }
+        uint32_t x[2][32];
+        prompt_ld32(s_at, x[0]);
+#pragma unroll 1
+        for (int h = 0; h < 4; h += 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                prompt_wait_ld();
+                if (k == 0) prompt_ld32(s_at + 32 * h + 32, x[1]);
+                else if (h < 2) prompt_ld32(s_at + 64, x[0]);
+                uint32_t w[16];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t* of = x[k] + 16 * g;
+                    if (masked) hide(of, visible - 32 * (h + k) - 16 * g);
+                    const int page = 2 * (h + k) + g;
+                    const float c = fmaxf(row_scale * plan.k_scale[page], kTiny), shift = plan.v_exp[page] + kHeadroom - u;
+                    const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
+                    uint64_t sums = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float a, b;
+                        unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        sums = add2(sums, pair(a, b));
+                        w[8 * g + i] = pack_half2(a, b);
+                    }
+                    float sum0, sum1;
+                    unpair(sums, sum0, sum1);
+                    l = fmaf(sum0 + sum1, ex2(-shift - m), l);                   // in units of m again
+                }
+                prompt_st16(s_at + 16 * (h + k), w);
+            }
+        }
+        prompt_wait_st();
+        prompt_fence_before();
+        __syncwarp();
+        if (lane == 0) prompt_arrive(bars + kbPFull + q);
+    }
+    if (ok && step) {
+        if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
+        ok = flags[0] == 0;
+        prompt_fence_after();
     }
     // The row's values: in units of the weights' reference, divided by their sum where this CTA saw all of them.
     const bool whole = p.chunks == 1;
@@ -433,7 +472,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
     if (whole && l != 0.f) f /= l;
     const bool nothing = job.token_a >= job.token_b || l == 0.f;
     const int* first_nan = reinterpret_cast<const int*>(smem + Smem::kNan);
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < D / 32; ++h) {
         uint32_t x[32];
         if (job.token_a < job.token_b && ok) {
@@ -505,20 +544,25 @@ __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, ui
 template <int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const Attend8Params p, int bf16) {
     using Smem = PromptSmem<D>;
-    extern __shared__ __align__(1024) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
     volatile int* flags = reinterpret_cast<volatile int*>(smem + Smem::kFlags);
     const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bars + kbKFull + i, 4);
+            mbar_init(bars + kbKFull + i, 2);
             mbar_init(bars + kbKEmpty + i, 1);
-            mbar_init(bars + kbVFull + i, 4);
+            mbar_init(bars + kbVFull + i, 2);
             mbar_init(bars + kbVEmpty + i, 1);
             mbar_init(bars + kbSFull + i, 1);
             mbar_init(bars + kbPFull + i, 4);
             mbar_init(bars + kbPvDone + i, 1);
         }
+        mbar_init(bars + kbRawKFull, 1);
+        mbar_init(bars + kbRawKEmpty, 2);
+        mbar_init(bars + kbRawVFull, 1);
+        mbar_init(bars + kbRawVEmpty, 2);
+        for (int i = 0; i < kPlans; ++i) mbar_init(bars + kbPlanEmpty + i, 1);
         flags[0] = flags[1] = 0;
         fence_barrier_init();
     }
@@ -568,10 +612,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Smem::kTmemSlot);
     if (warp < 8) {
         if (warp < 4 * job.tiles) prompt_softmax<D>(p, job, split, smem, bars, flags, tmem, bf16 != 0, row_scale);
+    } else if (warp < 10) {
+        prompt_convert<D, false>(job, smem, bars, flags);
     } else if (warp < 12) {
-        prompt_convert<D>(p, job, seq, smem, bars, flags);
-    } else if ((tid & 31) == 0 && job.token_a < job.token_b) {
-        prompt_multiply<D>(job, smem, bars, flags, tmem);
+        prompt_convert<D, true>(job, smem, bars, flags);
+    } else if (warp == 13) {
+        prompt_plan<D>(p, job, seq, smem, bars, flags);
+    } else if (job.token_a < job.token_b) {
+        prompt_multiply<D>(job, smem, bars, flags);
     }
     __syncwarp();
     if (flags[0] && p.status && (tid & 31) == 0) atomicOr(p.status, TQ_STATUS_TIMEOUT);

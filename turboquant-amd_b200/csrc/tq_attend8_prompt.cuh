@@ -3,13 +3,14 @@
 // A CTA takes 256 query rows (two tiles of 128; rows are token-major, the heads of a group side by side) of one sequence and KV head
 // and walks over the keys, 128 tokens at a time:
 //
-//   planner warp 13       looks up the blocks and scales of the tiles to come and has their codes copied into shared memory (bulk copies,
+//   planner warp          looks up the blocks and scales of the tiles to come and has their codes copied into shared memory (bulk copies,
 //                         2 KB of a page each)
-//   converter warps       8, 9: keys, 10, 11: values: codes to fp16 - exact, whatever the scale - as operands in shared memory, K K-major,
+//   converter warps       two for keys, two for values: codes to fp16 - exact, whatever the scale - as operands in shared memory, K K-major,
 //                         V MN-major.  (A product in e4m3 itself would need queries and weights as sums of two or three e4m3 terms,
 //                         which costs more)
-//   MMA warp 12           one thread: S_q = Q_q K^T (shared x shared), O_q += P_q V (tensor memory x shared), q = 0, 1
-//   softmax warps 0-3, 4-7  thread = query row of tile 0 / 1: maximum, weights in fp16 back into the columns of S, sums
+//   product warp          one thread: S_q = Q_q K^T (shared x shared), O_q += P_q V (tensor memory x shared), q = 0, 1
+//   softmax warps         two threads for each query row, 64 columns each: weights in fp16 back into columns of S, sums.  (With one
+//                         thread a row, two warps a scheduler, their latencies were not covered: 2800 cycles a tile)
 //
 // The two tiles take turns: while one's weights are computed, the tensor cores work on the other's products.  The references of the softmax
 // are raised only when a score passes them by 2^8, so that O in tensor memory is rarely rescaled.  Bound: the exponentials (16 a cycle
@@ -28,7 +29,9 @@
 namespace tq {
 namespace {
 
-constexpr int kPromptThreads = 14 * 32;
+// Warps: 0-3 and 4-7 the weights of query tile 0 (columns 0-63, 64-127), 8-11 and 12-15 of tile 1, 16, 17 keys, 18, 19 values, 20 products, 21 planner.
+constexpr int kSoftmaxWarps = 16;
+constexpr int kPromptThreads = (kSoftmaxWarps + 6) * 32;
 constexpr int kTile = 128;                      // query rows of a tile, and tokens of a step
 constexpr int kTilePages = kTile / kPageTokens;
 constexpr int kPlans = 8;
@@ -47,13 +50,15 @@ struct PromptSmem {
     static constexpr int kFlags = 260;                                   // failed, NaN seen
     static constexpr int kPlan = 272;
     static constexpr int kNan = kPlan + kPlans * sizeof(StepPlan);       // [D] first token with a NaN in this dim of V
-    static constexpr int kQ = 2048;                                      // [2]
+    static constexpr int kOver = kNan + D * 4;                           // [2 steps][8 pairs of warps][2] a score passes its reference
+    static constexpr int kRows = kOver + 2 * 8 * 2 * 4;                  // [8 pairs][32] one value of a row, from thread to thread
+    static constexpr int kQ = 2688;                                      // [2]
     static constexpr int kK = kQ + 2 * kOperand;                         // [2]
     static constexpr int kV = kK + 2 * kOperand;                         // [2]
     static constexpr int kRawK = kV + 2 * kOperand;                      // codes of a tile's keys, values
     static constexpr int kRawV = kRawK + kTile * D;
     static constexpr int kBytes = kRawV + kTile * D;
-    static_assert(kNan + D * 4 <= kQ && kBytes <= 227 * 1024, "shared memory map");
+    static_assert(kRows + 8 * 32 * 4 <= kQ && kBytes <= 227 * 1024, "shared memory map");
 };
 
 enum PromptBar { kbKFull = 0, kbKEmpty = 2, kbVFull = 4, kbVEmpty = 6, kbSFull = 8, kbPFull = 10, kbPvDone = 12, kbRawKFull = 14, kbRawKEmpty = 15, kbRawVFull = 16, kbRawVEmpty = 17,
@@ -87,20 +92,19 @@ __device__ __forceinline__ void prompt_mma_ts(uint32_t d, uint32_t a, uint64_t b
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
 }
-__device__ __forceinline__ void prompt_ld32(uint32_t at, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(at) : "memory");
-}
 __device__ __forceinline__ void prompt_ld16(uint32_t at, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(at) : "memory");
+}
+__device__ __forceinline__ void prompt_st32(uint32_t at, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 __device__ __forceinline__ void prompt_st16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -294,7 +298,7 @@ __device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* b
     auto products = [&](int q, int s, uint32_t accumulate) {
 #pragma unroll
         for (int i = 0; i < kTile / 16; ++i)
-            prompt_mma_ts(2 * kTile + q * kTile, q * kTile + i * 8, values + (s * Smem::kOperand + i * 2 * (D * 16)) / 16, kOut, i ? 1u : accumulate);
+            prompt_mma_ts(2 * kTile + q * kTile, q * kTile + i / 4 * 64 + i % 4 * 8, values + (s * Smem::kOperand + i * 2 * (D * 16)) / 16, kOut, i ? 1u : accumulate);
         prompt_commit(bars + kbPvDone + q);
     };
     if (!wait(kbKFull, 0)) return;
@@ -353,17 +357,34 @@ __device__ __forceinline__ void hide(uint32_t* x, int visible) {
         if (i >= visible) x[i] = 0xff800000u;
 }
 
+// A value of the other thread of this row.  The pair's warps meet at a barrier of their own before and after.
+__device__ __forceinline__ float exchange(float* row, int half, int barrier, float mine) {
+    float theirs = 0.f;
+    if (half) *row = mine;
+    asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory");
+    if (!half) {
+        theirs = *row;
+        *row = mine;
+    }
+    asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory");
+    if (half) theirs = *row;
+    asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory");
+    return theirs;
+}
+
 template <int D>
 __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int split, uint8_t* smem, uint64_t* bars, volatile int* flags, uint32_t tmem,
                                bool bf16, float row_scale) {
     using Smem = PromptSmem<D>;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = warp >> 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = warp >> 3, half = warp >> 2 & 1, together = q * 4 + (warp & 3);
     const int row = job.r0 + q * kTile + (warp & 3) * 32 + lane;
     const int limit = job.len - job.nq + min(row, job.nrows - 1) / p.group + 1;
     const int warp_limit = __reduce_min_sync(0xffffffffu, limit);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + q * kTile, o_at = tmem + lanes + 2 * kTile + q * kTile;
+    const uint32_t s_at = tmem + lanes + q * kTile + 64 * half, o_at = tmem + lanes + 2 * kTile + q * kTile + D / 2 * half;
     const StepPlan* plans = reinterpret_cast<const StepPlan*>(smem + Smem::kPlan);
+    volatile int* over = reinterpret_cast<volatile int*>(smem + Smem::kOver) + together * 2;
+    float* row_slot = reinterpret_cast<float*>(smem + Smem::kRows) + together * 32 + lane;
     float m = kNothing, u = kNothing, l = 0.f;
     bool ok = true;
     int step = 0;
@@ -371,34 +392,57 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
         // the plan was written before the codes of V were asked for
         if (!mbar_wait_bounded(bars + kbSFull + q, step & 1)) flags[0] = 1;
         if (!mbar_wait_bounded(bars + kbVFull + (step & 1), step >> 1 & 1)) flags[0] = 1;
-        if (flags[0]) {
-            ok = false;
-            break;
-        }
         prompt_fence_after();
         const StepPlan& plan = plans[step % kPlans];
+        const int visible = limit - token0 - 64 * half;
         const bool masked = token0 + kTile > warp_limit;
-        const int visible = limit - token0;
-        float most = kNothing, most_v = kNothing;
-#pragma unroll 1
-        for (int h = 0; h < 4; h += 2) {
-            uint32_t x[2][32];
-            prompt_ld32(s_at + 32 * h, x[0]);
-            prompt_ld32(s_at + 32 * h + 32, x[1]);
-            prompt_wait_ld();
+        // Weights are computed against the references as they are, and the largest scores on the way.  Only where these pass the
+        // references - always at first - the references are raised, and the scores, which are still there, gone through again.
+        float sum;
+        uint32_t w[32];
+        for (bool again = false;; again = true) {
+            float most = kNothing, most_v = kNothing;
+            sum = 0.f;
+            uint32_t x[2][16];
+            prompt_ld16(s_at, x[0]);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                uint32_t* of = x[g >> 1] + 16 * (g & 1);
-                if (masked) hide(of, visible - 32 * h - 16 * g);
-                float a = __uint_as_float(of[0]);
+                uint32_t(&of)[16] = x[g & 1];
+                prompt_wait_ld();
+                if (g < 3) prompt_ld16(s_at + 16 * g + 16, x[(g + 1) & 1]);
+                if (masked) hide(of, visible - 16 * g);
+                const float c = fmaxf(row_scale * plan.k_scale[4 * half + g], kTiny), ev = plan.v_exp[4 * half + g], shift = ev + kHeadroom - u;
+                float a = fmaxf(fmaxf(__uint_as_float(of[0]), __uint_as_float(of[1])), __uint_as_float(of[2]));
 #pragma unroll
-                for (int i = 1; i < 15; i += 2) a = fmaxf(fmaxf(a, __uint_as_float(of[i])), __uint_as_float(of[i + 1]));
-                a = fmaxf(a, __uint_as_float(of[15])) * fmaxf(row_scale * plan.k_scale[2 * h + g], kTiny);
+                for (int i = 3; i < 15; i += 2) a = fmaxf(fmaxf(a, __uint_as_float(of[i])), __uint_as_float(of[i + 1]));
+                a = fmaxf(a, __uint_as_float(of[15])) * c;
                 most = fmaxf(most, a);
-                most_v = fmaxf(most_v, a + plan.v_exp[2 * h + g]);
+                most_v = fmaxf(most_v, a + ev);
+                const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
+                uint64_t sums = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float y, z;
+                    unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
+                    y = ex2(y);
+                    z = ex2(z);
+                    sums = add2(sums, pair(y, z));
+                    w[8 * g + i] = pack_half2(y, z);
+                }
+                float sum0, sum1;
+                unpair(sums, sum0, sum1);
+                sum = fmaf(sum0 + sum1, ex2(-shift - m), sum);               // in units of m again
             }
-        }
-        if (__any_sync(0xffffffffu, most > m + kLazy || most_v > u + kLazy)) {
+            if (again) break;
+            // Both warps of the rows decide alike, also about giving up.
+            const int mine = __any_sync(0xffffffffu, most > m + kLazy || most_v > u + kLazy) ? 1 : 0;
+            if (lane == 0) over[(step & 1) * 16 + half] = mine | (flags[0] ? 2 : 0);
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + together) : "memory");
+            const int both = over[(step & 1) * 16] | over[(step & 1) * 16 + 1];
+            if (both & 2) ok = false;
+            if (both != 1) break;
+            most = fmaxf(most, exchange(row_slot, half, 1 + together, most));
+            most_v = fmaxf(most_v, exchange(row_slot, half, 1 + together, most_v));
             const float m1 = fmaxf(m, most), u1 = fmaxf(u, most_v);
             l *= ex2(m - m1);
             const float down = ex2(u - u1);
@@ -409,50 +453,18 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
                 if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
                 prompt_fence_after();
 #pragma unroll 1
-                for (int h = 0; h < D / 16; ++h) {
-                    uint32_t o[16];
-                    prompt_ld16(o_at + 16 * h, o);
+                for (int h = 0; h < D / 32; ++h) {
+                    prompt_ld16(o_at + 16 * h, x[0]);
                     prompt_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
-                    prompt_st16(o_at + 16 * h, o);
+                    for (int i = 0; i < 16; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * down);
+                    prompt_st16(o_at + 16 * h, x[0]);
                 }
             }
         }
-        uint32_t x[2][32];
-        prompt_ld32(s_at, x[0]);
-#pragma unroll 1
-        for (int h = 0; h < 4; h += 2) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                prompt_wait_ld();
-                if (k == 0) prompt_ld32(s_at + 32 * h + 32, x[1]);
-                else if (h < 2) prompt_ld32(s_at + 64, x[0]);
-                uint32_t w[16];
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    uint32_t* of = x[k] + 16 * g;
-                    if (masked) hide(of, visible - 32 * (h + k) - 16 * g);
-                    const int page = 2 * (h + k) + g;
-                    const float c = fmaxf(row_scale * plan.k_scale[page], kTiny), shift = plan.v_exp[page] + kHeadroom - u;
-                    const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
-                    uint64_t sums = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float a, b;
-                        unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), a, b);
-                        a = ex2(a);
-                        b = ex2(b);
-                        sums = add2(sums, pair(a, b));
-                        w[8 * g + i] = pack_half2(a, b);
-                    }
-                    float sum0, sum1;
-                    unpair(sums, sum0, sum1);
-                    l = fmaf(sum0 + sum1, ex2(-shift - m), l);                   // in units of m again
-                }
-                prompt_st16(s_at + 16 * (h + k), w);
-            }
-        }
+        if (!ok) break;
+        l += sum;
+        prompt_st32(s_at, w);
         prompt_wait_st();
         prompt_fence_before();
         __syncwarp();
@@ -460,12 +472,13 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
     }
     if (ok && step) {
         if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
-        ok = flags[0] == 0;
         prompt_fence_after();
     }
+    ok = ok && flags[0] == 0;
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + together) : "memory");
+    l += exchange(row_slot, half, 1 + together, l);
     // The row's values: in units of the weights' reference, divided by their sum where this CTA saw all of them.
-    const bool whole = p.chunks == 1;
-    const bool store = ok && row < job.nrows;
+    const bool whole = p.chunks == 1, store = ok && row < job.nrows;
     const int token = row / p.group, head = job.kvh * p.group + row - token * p.group;
     const int64_t at = static_cast<int64_t>(job.first_row + token) * p.q_heads + head;
     float f = l == 0.f ? 0.f : ex2(u - m - kHeadroom);
@@ -474,70 +487,83 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
     const int* first_nan = reinterpret_cast<const int*>(smem + Smem::kNan);
 #pragma unroll 1
     for (int h = 0; h < D / 32; ++h) {
-        uint32_t x[32];
+        const int d0 = D / 2 * half + 16 * h;
+        uint32_t x[16];
         if (job.token_a < job.token_b && ok) {
-            prompt_ld32(o_at + 32 * h, x);
+            prompt_ld16(o_at + 16 * h, x);
             prompt_wait_ld();
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = nothing ? 0u : __float_as_uint(__uint_as_float(x[i]) * f);
+        for (int i = 0; i < 16; ++i) x[i] = nothing ? 0u : __float_as_uint(__uint_as_float(x[i]) * f);
         if (flags[1]) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (first_nan[32 * h + i] < limit) x[i] = 0x7fffffffu;
+            for (int i = 0; i < 16; ++i)
+                if (first_nan[d0 + i] < limit) x[i] = 0x7fffffffu;
         }
         if (!store) continue;
         if (whole) {
-            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at * D + 32 * h);
+            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at * D + d0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t w[4];
+            for (int i = 0; i < 2; ++i) {
+                uint32_t v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = pack_out(__uint_as_float(x[8 * i + 2 * j]), __uint_as_float(x[8 * i + 2 * j + 1]), bf16);
-                to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int j = 0; j < 4; ++j) v[j] = pack_out(__uint_as_float(x[8 * i + 2 * j]), __uint_as_float(x[8 * i + 2 * j + 1]), bf16);
+                to[i] = make_uint4(v[0], v[1], v[2], v[3]);
             }
         } else {
-            float2* to = reinterpret_cast<float2*>(p.partials + (at * p.chunks + split) * (D + 2) + 32 * h);
+            float2* to = reinterpret_cast<float2*>(p.partials + (at * p.chunks + split) * (D + 2) + d0);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to[i] = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+            for (int i = 0; i < 8; ++i) to[i] = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
         }
     }
-    if (store && !whole) *reinterpret_cast<float2*>(p.partials + (at * p.chunks + split) * (D + 2) + D) = make_float2(m, l);
+    if (store && !whole && !half) *reinterpret_cast<float2*>(p.partials + (at * p.chunks + split) * (D + 2) + D) = make_float2(m, l);
 }
 
-// Queries of a tile as K-major A operand, thread = row; returns the factor of its scores in units of log2.
+// Queries of a tile as K-major A operand, two threads a row; returns the factor of its scores in units of log2.  All threads of the block
+// come here (a row's largest value is looked for by both of its threads), those of no row with row = -1.
 template <int D>
 __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, uint8_t* smem, bool bf16) {
     using Smem = PromptSmem<D>;
-    const int q = threadIdx.x / kTile, r = threadIdx.x % kTile, row = job.r0 + threadIdx.x;
-    uint32_t x[D / 2];
-    if (row < job.nrows) {
+    constexpr int kWords = D / 4;
+    const int warp = threadIdx.x >> 5, q = warp >> 3, half = warp >> 2 & 1, r = threadIdx.x & (kTile - 1), row = job.r0 + q * kTile + r;
+    const bool mine = warp < 8 * job.tiles;
+    uint32_t* largest = reinterpret_cast<uint32_t*>(smem + Smem::kK);       // not in use yet
+    uint32_t x[kWords];
+    uint32_t most = 0;
+    if (mine && row < job.nrows) {
         const int token = row / p.group, head = job.kvh * p.group + row - token * p.group;
-        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(job.first_row + token) * p.q_heads + head) * D);
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(job.first_row + token) * p.q_heads + head) * D +
+                                                           D / 2 * half);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
+        for (int i = 0; i < kWords / 4; ++i) {
             const uint4 w = __ldg(from + i);
             x[4 * i] = w.x; x[4 * i + 1] = w.y; x[4 * i + 2] = w.z; x[4 * i + 3] = w.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) x[i] = 0;
+        for (int i = 0; i < kWords; ++i) x[i] = 0;
     }
-    float row_scale = fabsf(p.scale_log2);
     if (bf16) {      // into the range of fp16 by a power of two, as in load_queries
-        uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) most = max(most, max(x[i] & 0x7fffu, x[i] >> 16 & 0x7fffu));
+        for (int i = 0; i < kWords; ++i) most = max(most, max(x[i] & 0x7fffu, x[i] >> 16 & 0x7fffu));
+        if (mine) largest[threadIdx.x] = most;
+        __syncthreads();
+        if (mine) most = max(most, largest[threadIdx.x ^ kTile]);
+        __syncthreads();
+    }
+    if (!mine) return 0.f;
+    float row_scale = fabsf(p.scale_log2);
+    if (bf16) {
         const int e = min(max(static_cast<int>(most >> 7) - 127, -120), 120);
         const float down = exp2_int(-e);
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) x[i] = pack_half2(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down);
+        for (int i = 0; i < kWords; ++i) x[i] = pack_half2(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down);
         row_scale *= exp2_int(e);
     }
     const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-    const uint32_t to = smem_u32(smem) + Smem::kQ + q * Smem::kOperand + r * 16;
+    const uint32_t to = smem_u32(smem) + Smem::kQ + q * Smem::kOperand + r * 16 + half * (D / 16) * 2048;
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) sts16(to + i * 2048, x[4 * i] ^ sign, x[4 * i + 1] ^ sign, x[4 * i + 2] ^ sign, x[4 * i + 3] ^ sign);
+    for (int i = 0; i < kWords / 4; ++i) sts16(to + i * 2048, x[4 * i] ^ sign, x[4 * i + 1] ^ sign, x[4 * i + 2] ^ sign, x[4 * i + 3] ^ sign);
     return row_scale;
 }
 
@@ -555,7 +581,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
             mbar_init(bars + kbVFull + i, 2);
             mbar_init(bars + kbVEmpty + i, 1);
             mbar_init(bars + kbSFull + i, 1);
-            mbar_init(bars + kbPFull + i, 4);
+            mbar_init(bars + kbPFull + i, 8);
             mbar_init(bars + kbPvDone + i, 1);
         }
         mbar_init(bars + kbRawKFull, 1);
@@ -597,26 +623,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
     job.token_a = min(split * each * kTile, most);
     job.token_b = min((split + 1) * each * kTile, most);
 
-    if (warp == 12) {
+    if (warp == kSoftmaxWarps + 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem) + Smem::kTmemSlot), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    float row_scale = 0.f;
-    if (warp < 4 * job.tiles) {
-        row_scale = prompt_queries<D>(p, job, smem, bf16 != 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
+    const float row_scale = prompt_queries<D>(p, job, smem, bf16 != 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     prompt_fence_before();
     __syncthreads();
     prompt_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Smem::kTmemSlot);
-    if (warp < 8) {
-        if (warp < 4 * job.tiles) prompt_softmax<D>(p, job, split, smem, bars, flags, tmem, bf16 != 0, row_scale);
-    } else if (warp < 10) {
+    if (warp < kSoftmaxWarps) {
+        if (warp < 8 * job.tiles) prompt_softmax<D>(p, job, split, smem, bars, flags, tmem, bf16 != 0, row_scale);
+    } else if (warp < kSoftmaxWarps + 2) {
         prompt_convert<D, false>(job, smem, bars, flags);
-    } else if (warp < 12) {
+    } else if (warp < kSoftmaxWarps + 4) {
         prompt_convert<D, true>(job, smem, bars, flags);
-    } else if (warp == 13) {
+    } else if (warp == kSoftmaxWarps + 5) {
         prompt_plan<D>(p, job, seq, smem, bars, flags);
     } else if (job.token_a < job.token_b) {
         prompt_multiply<D>(job, smem, bars, flags);
@@ -625,7 +648,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
     if (flags[0] && p.status && (tid & 31) == 0) atomicOr(p.status, TQ_STATUS_TIMEOUT);
     prompt_fence_before();
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == kSoftmaxWarps + 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 }  // namespace

@@ -46,9 +46,9 @@ template <int D>
 struct PromptSmem {
     static constexpr int kOperand = kTile * D * 2;                       // bytes of a tile of queries, keys or values
     static constexpr int kBars = 0;
-    static constexpr int kTmemSlot = 256;
-    static constexpr int kFlags = 260;                                   // failed, NaN seen
-    static constexpr int kPlan = 272;
+    static constexpr int kTmemSlot = 288;
+    static constexpr int kFlags = 292;                                   // failed, NaN seen
+    static constexpr int kPlan = 304;
     static constexpr int kNan = kPlan + kPlans * sizeof(StepPlan);       // [D] first token with a NaN in this dim of V
     static constexpr int kOver = kNan + D * 4;                           // [2 steps][8 pairs of warps][2] a score passes its reference
     static constexpr int kRows = kOver + 2 * 8 * 2 * 4;                  // [8 pairs][32] one value of a row, from thread to thread
@@ -62,8 +62,8 @@ struct PromptSmem {
 };
 
 enum PromptBar { kbKFull = 0, kbKEmpty = 2, kbVFull = 4, kbVEmpty = 6, kbSFull = 8, kbPFull = 10, kbPvDone = 12, kbRawKFull = 14, kbRawKEmpty = 15, kbRawVFull = 16, kbRawVEmpty = 17,
-                 kbPlanEmpty = 18, kbBars = 18 + kPlans };
-static_assert(kbBars * 8 <= 256, "barriers");
+                 kbPlanFull = 18, kbPlanEmpty = 18 + kPlans, kbBars = 18 + 2 * kPlans };
+static_assert(kbBars * 8 <= 288, "barriers");
 
 __device__ __forceinline__ void prompt_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -200,7 +200,10 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
             plan.last = token0 + kTile >= job.token_b;
         }
         __syncwarp();
-        if (lane == 0) mbar_expect_tx(bars + kbRawVFull, count * kPart);       // tells of the plan, too: its writes come before
+        if (lane == 0) {
+            prompt_arrive(bars + kbPlanFull + slot);
+            mbar_expect_tx(bars + kbRawVFull, count * kPart);
+        }
         __syncwarp();
         if (here && lane >= 8 && lane < 16) bulk_g2s(smem + Smem::kRawV + mine * kPart, at + kPart, kPart, bars + kbRawVFull);
     }
@@ -285,6 +288,7 @@ __device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* b
     const bool both = __shfl_sync(0xffffffffu, job.tiles, 0) == 2;
     auto wait = [&](int bar, uint32_t parity) {
         if (!mbar_wait_bounded(bars + bar, parity)) flags[0] = 1;
+        __syncwarp();
         return flags[0] == 0;
     };
     const uint64_t queries = prompt_desc(base + Smem::kQ, 2048, 128), keys = prompt_desc(base + Smem::kK, 2048, 128),
@@ -389,9 +393,9 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
     bool ok = true;
     int step = 0;
     for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
-        // the plan was written before the codes of V were asked for
+        if (!mbar_wait_bounded(bars + kbPlanFull + step % kPlans, step / kPlans & 1)) flags[0] = 1;
         if (!mbar_wait_bounded(bars + kbSFull + q, step & 1)) flags[0] = 1;
-        if (!mbar_wait_bounded(bars + kbVFull + (step & 1), step >> 1 & 1)) flags[0] = 1;
+        __syncwarp();                                                        // what follows is for whole warps
         prompt_fence_after();
         const StepPlan& plan = plans[step % kPlans];
         const int visible = limit - token0 - 64 * half;
@@ -437,6 +441,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
             // Both warps of the rows decide alike, also about giving up.
             const int mine = __any_sync(0xffffffffu, most > m + kLazy || most_v > u + kLazy) ? 1 : 0;
             if (lane == 0) over[(step & 1) * 16 + half] = mine | (flags[0] ? 2 : 0);
+            __syncwarp();
             asm volatile("bar.sync %0, 64;" ::"r"(1 + together) : "memory");
             const int both = over[(step & 1) * 16] | over[(step & 1) * 16 + 1];
             if (both & 2) ok = false;
@@ -451,6 +456,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
             if (step) {
                 // O is whole when the product of the step before is done
                 if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
+                __syncwarp();
                 prompt_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < D / 32; ++h) {
@@ -474,6 +480,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
         if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
         prompt_fence_after();
     }
+    __syncwarp();
     ok = ok && flags[0] == 0;
     asm volatile("bar.sync %0, 64;" ::"r"(1 + together) : "memory");
     l += exchange(row_slot, half, 1 + together, l);
@@ -588,7 +595,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
         mbar_init(bars + kbRawKEmpty, 2);
         mbar_init(bars + kbRawVFull, 1);
         mbar_init(bars + kbRawVEmpty, 2);
-        for (int i = 0; i < kPlans; ++i) mbar_init(bars + kbPlanEmpty + i, 1);
+        for (int i = 0; i < kPlans; ++i) {
+            mbar_init(bars + kbPlanFull + i, 1);
+            mbar_init(bars + kbPlanEmpty + i, 1);
+        }
         flags[0] = flags[1] = 0;
         fence_barrier_init();
     }

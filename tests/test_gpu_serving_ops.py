@@ -288,6 +288,14 @@ def test_one_long_sequence(D, Hq, H, dtype):
     _check_attention(gen(7), [5003], [1], Hq, H, D, 16, dtype, max_seq_len=5003)
 
 
+@pytest.mark.parametrize("n,H,L", [(1, 1, 17), (1, 1, 300), (2, 4, 130), (5, 4, 600), (14, 5, 40), (19, 8, 33), (150, 1, 70)])
+@pytest.mark.parametrize("G", [1, 8, 11])
+def test_clusters_of_every_size(n, H, L, G):
+    """Few items with clusters of 8, 4 and 2 CTAs, and of one, some of whose warps and CTAs have no page."""
+    lens = [max(0, L - 13 * i) for i in range(n)]
+    _check_attention(gen(n), lens, [1] * n, G * H, H, 128 if G > 1 else 64, 16, torch.float16)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("D,Hq,H,bs", [(128, 8, 2, 16), (64, 5, 1, 32), (128, 16, 1, 16), (128, 3, 3, 32)])
 def test_several_queries_per_sequence(D, Hq, H, bs, dtype):
@@ -305,24 +313,24 @@ def test_prompt_chunks(queries, lens, D, Hq, H):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("D,Hq,H,bs", [(128, 8, 1, 16), (64, 10, 2, 32), (128, 16, 1, 48), (64, 16, 1, 16), (128, 12, 6, 16)])
 def test_wide_tables_single_queries(D, Hq, H, bs, dtype):
-    _check_attention(gen(Hq), [0, 1, 15, 16, 17, 31, 33, 64, 100, 257, 1000, -3, 2], [1] * 13, Hq, H, D, bs, dtype, width=512)
+    _check_attention(gen(Hq), [0, 1, 15, 16, 17, 31, 33, 64, 100, 257, 1000, -3, 2], [1] * 13, Hq, H, D, bs, dtype, width=3000)
 
 
 @pytest.mark.parametrize("lens", [[1], [0, 0, 0], [5003, 0, 0, 7], [16 * 2368 // 4], [16 * 2368 // 4 + 1, 1], [40] * 700, list(range(0, 1400, 3))])
 @pytest.mark.parametrize("D,Hq,H", [(128, 8, 1), (64, 12, 4)])
 def test_wide_tables_shares(lens, D, Hq, H):
     """Fewer pages than warps, one more than evenly shared, more sequences than entries of the prefix, shares of many items."""
-    _check_attention(gen(len(lens)), lens, [1] * len(lens), Hq, H, D, 16, torch.float16, width=5000 // len(lens) + 1200)
+    _check_attention(gen(len(lens)), lens, [1] * len(lens), Hq, H, D, 16, torch.float16, width=40000 // len(lens) + 1200)
 
 
 @pytest.mark.parametrize("D,Hq,H,bs", [(128, 8, 2, 16), (64, 5, 1, 32), (128, 16, 1, 16), (128, 3, 3, 32)])
 def test_wide_tables_several_queries(D, Hq, H, bs):
     lens, queries = [40, 1, 300, 17, 0, 2, 64, 33, 700], [4, 1, 7, 0, 3, 5, 6, 2, 8]
-    _check_attention(gen(Hq), lens, queries, Hq, H, D, bs, torch.bfloat16, width=600)
+    _check_attention(gen(Hq), lens, queries, Hq, H, D, bs, torch.bfloat16, width=4000)
 
 
 def test_negative_and_zero_scales():
-    for width in (0, 1300):
+    for width in (0, 9000):
         _check_attention(gen(5), [300, 40], [1, 1], 8, 2, 128, 16, torch.float16, sm_scale=-0.05, width=width)
         _check_attention(gen(6), [300, 40], [1, 1], 8, 2, 128, 16, torch.bfloat16, sm_scale=0.0, width=width)
 

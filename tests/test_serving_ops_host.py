@@ -159,8 +159,8 @@ def test_cache8_calls_refuse_without_touching_a_gpu():
     assert attend(q=NULL) == attend(tables=NULL) == attend(blocks=0) == attend(hq=7) == attend(most=0) == attend(T=1) == attend(most=2) == -1
     assert attend(q=at(8)) == attend(out=at(8)) == attend(cache=at(8)) == -1
     assert attend(dtype=2) == attend(D=96) == attend(bs=8) == attend(pages=(1 << 27)) == -2
-    assert attend(T=1, ns=1, pages=256) == -4                              # split over the GPU, and no workspace
-    need = L.tq_attend8_workspace_bytes(1, 1, 8, 2, 128, 1, 256)
+    assert attend(T=1, ns=1, pages=8192) == -4                             # shared out over the GPU, and no workspace
+    need = L.tq_attend8_workspace_bytes(1, 1, 8, 2, 128, 1, 8192)
     assert need > 0 and L.tq_attend8_workspace_bytes(0, 0, 8, 2, 128, 1, 256) == 0
     assert L.tq_attend8_workspace_bytes(1, 1, 8, 3, 128, 1, 256) == -1 and L.tq_attend8_workspace_bytes(1, 1, 8, 2, 96, 1, 256) == -2
 

@@ -22,7 +22,7 @@ struct Attend8Params {
     int32_t* status;
     int64_t num_blocks, table_stride;
     float scale_log2;
-    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, tile_rows, chunk_pages, chunks, merge_blocks, zero_tail;
+    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, chunks, merge_blocks, zero_tail;
 };
 
 constexpr float kNothing = -3e38f;      // reference of a row that has seen no token: below every score, and finite, so that differences are numbers
@@ -87,13 +87,18 @@ __device__ __forceinline__ void load_values(Page<D>& x, const uint8_t* base, int
 
 // Query rows r0 .. r0 + 8 NT of a sequence as B operands.  fp16 queries are used as they are; bf16 ones are brought into the range of
 // fp16 by a power of two for each row, which costs no bit of values within 2^-14 of the row's largest.
-template <int D, int NT, bool BF16>
-__device__ __forceinline__ void load_queries(Rows<D, NT>& w, const Attend8Params& p, int first_row, int kvh, int r0, int nrows, int len, int nq, int lane) {
+template <int D, int NT>
+struct QueryWords {
+    uint32_t x[NT][D / 64][8];
+};
+
+template <int D, int NT>
+__device__ __forceinline__ void ask_queries(QueryWords<D, NT>& w, const Attend8Params& p, int first_row, int kvh, int r0, int nrows, int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = r0 + 8 * n + g;
-        uint32_t x[D / 64][8];
+        uint32_t(&x)[D / 64][8] = w.x[n];
         if (r < nrows) {
             const int token = r / p.group, head = kvh * p.group + r - token * p.group;
             const uint16_t* src = static_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(first_row + token) * p.q_heads + head) * D + 16 * t;
@@ -109,6 +114,15 @@ __device__ __forceinline__ void load_queries(Rows<D, NT>& w, const Attend8Params
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[c][i] = 0;
         }
+    }
+}
+
+template <int D, int NT, bool BF16>
+__device__ __forceinline__ void set_queries(Rows<D, NT>& w, QueryWords<D, NT>& words, const Attend8Params& p, int r0, int nrows, int len, int nq, int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        uint32_t(&x)[D / 64][8] = words.x[n];
         float row_scale = fabsf(p.scale_log2);
         if (p.scale_log2 < 0.f) {
 #pragma unroll
@@ -157,6 +171,13 @@ __device__ __forceinline__ void load_queries(Rows<D, NT>& w, const Attend8Params
             for (int j = 0; j < 4; ++j) w.o[i][n][j] = 0.f;
     w.min_limit = len - nq + r0 / p.group + 1;
     w.max_limit = len - nq + min(r0 + 8 * NT - 1, nrows - 1) / p.group + 1;
+}
+
+template <int D, int NT, bool BF16>
+__device__ __forceinline__ void load_queries(Rows<D, NT>& w, const Attend8Params& p, int first_row, int kvh, int r0, int nrows, int len, int nq, int lane) {
+    QueryWords<D, NT> words;
+    ask_queries<D, NT>(words, p, first_row, kvh, r0, nrows, lane);
+    set_queries<D, NT, BF16>(w, words, p, r0, nrows, len, nq, lane);
 }
 
 template <int D, int NT>
@@ -315,12 +336,41 @@ __device__ __forceinline__ void page_products(Rows<D, NT>& w, const Page<D>& x, 
                 if (found[i][n][j] > 0.f) w.o[i][n][j] = __uint_as_float(0x7fffffffu);
 }
 
+constexpr int kMaxCluster = 8;
+
+__device__ __forceinline__ uint32_t cluster_address(uint32_t at, int cta) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(cta));
+    return r;
+}
+__device__ __forceinline__ float2 load_cluster2(uint32_t at) {
+    float2 x;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+    return x;
+}
+
+__device__ __forceinline__ uint32_t pack_out(float a, float b, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return pack_half2(a, b);
+}
+
+// A query row's output from its D / 32 sums of each lane.
+template <int D, bool BF16>
+__device__ __forceinline__ void store_row(const Attend8Params& p, int first_row, int kvh, int row, const float (&o)[D / 32], float l, int lane) {
+    const int token = row / p.group, head = kvh * p.group + row - token * p.group;
+    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + (static_cast<int64_t>(first_row + token) * p.q_heads + head) * D) + lane * (D / 64);
+    const float f = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) to[i] = l == 0.f ? 0u : pack_out(o[2 * i] * f, o[2 * i + 1] * f, BF16);
+}
+
 __device__ __forceinline__ void store_out(void* out, int64_t at, float x, bool bf16) {
     if (bf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(x);
     else static_cast<__half*>(out)[at] = __float2half_rn(x);
 }
-
-constexpr int kWarps = 4;
 
 // The rows of a sequence, inside the tensors whatever `starts` says; true when it has more than the launch is sized for, which are left out.
 __device__ __forceinline__ bool rows_of(const Attend8Params& p, int seq, int& first_row, int& nq) {
@@ -333,70 +383,80 @@ __device__ __forceinline__ bool rows_of(const Attend8Params& p, int seq, int& fi
     return n > p.max_queries;
 }
 
-// CTA: one chunk of pages of (sequence, KV head, tile of 8 NT query rows); its warps take a quarter of the pages each.
-template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32) attend8_kernel(const Attend8Params p) {
-    __shared__ float part_o[kWarps][8 * NT][D];
-    __shared__ float part_m[kWarps][8 * NT], part_l[kWarps][8 * NT];
+// Launches of few pages: a cluster of CTAs for each item (sequence, KV head, tile of 8 NT query rows), pages dealt out to the warps in
+// turn, so that which pages a warp has does not depend on the length, and length, block table and query are asked for together.  Parts are
+// joined in shared memory, those of the CTAs through distributed shared memory: a second kernel for that took as long as
+// the first (1 x 4096 tokens, 8 KV heads: 13.1 us with it).
+__host__ __device__ constexpr int few_smem(int d, int nt, int warps) { return warps * 8 * nt * (d + 2) * 4 + 8 * nt * (d + 2) * 4; }
+
+template <int D, int NT, bool BF16, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 && NT == 1 ? 4 : 1) attend8_few_kernel(const Attend8Params p) {
+    constexpr int COLS = 8 * NT;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* part_o = reinterpret_cast<float*>(smem);                 // [WARPS][COLS][D]
+    float* part_s = part_o + WARPS * COLS * D;                      // [WARPS][COLS][2]: reference, denominator
+    float* own_o = part_s + WARPS * COLS * 2;                       // [COLS][D], this CTA's
+    float* own_s = own_o + COLS * D;                                // [COLS][2]
     pdl_wait();
     pdl_release_if_small();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int g = lane >> 2, t = lane & 3;
-    // chunks of one item side by side, then the tiles of a KV head, which read the same pages
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     int rest = blockIdx.x;
-    const int chunk = rest % p.chunks;
+    const int part = rest % p.chunks;                               // of the item: CTA of the cluster
     rest /= p.chunks;
     const int tile = rest % p.tiles;
     rest /= p.tiles;
     const int kvh = rest % p.kv_heads, seq = rest / p.kv_heads;
+    const int32_t* table = p.tables + seq * p.table_stride;
+    const int first = part * WARPS + warp, stride = p.chunks * WARPS;
+    bool bad = false;
+    auto ask = [&](int page) { return page < p.max_pages ? __ldg(table + page / p.pages_per_block) : 0; };
+    int block = ask(first);
     if (p.zero_tail && blockIdx.x == 0) {
         const int64_t row = static_cast<int64_t>(p.q_heads) * D, used = p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs;
-        for (int64_t i = used * row + threadIdx.x; i < p.rows * row; i += kWarps * 32) static_cast<uint16_t*>(p.out)[i] = 0;
+        for (int64_t i = used * row + tid; i < p.rows * row; i += WARPS * 32) static_cast<uint16_t*>(p.out)[i] = 0;
     }
     int first_row, nq;
     const bool too_many = rows_of(p, seq, first_row, nq);
-    const int nrows = nq * p.group, r0 = tile * 8 * NT;
-    if (r0 >= nrows) return;
+    const int nrows = nq * p.group, r0 = tile * COLS;
+    if (r0 >= nrows) return;                                        // the whole cluster
     int len = p.seq_lens[seq];
+    QueryWords<D, NT> words;
+    ask_queries<D, NT>(words, p, first_row, kvh, r0, nrows, lane);
     const bool too_long = pages_of_length(len) > p.max_pages;
     if (too_long) len = p.max_pages * kPageTokens;
-    if ((too_long || too_many) && p.status && threadIdx.x == 0 && chunk == 0 && tile == 0 && kvh == 0)
+    if ((too_long || too_many) && p.status && tid == 0 && part == 0 && tile == 0 && kvh == 0)
         atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
-    Rows<D, NT> w;
-    load_queries<D, NT, BF16>(w, p, first_row, kvh, r0, nrows, len, nq, lane);
-    const int pages = pages_of_length(w.max_limit);
-    const int chunks = max((pages + p.chunk_pages - 1) / p.chunk_pages, 1);
-    if (chunk >= chunks) return;
-
-    const int c_a = chunk * p.chunk_pages, c_b = min(c_a + p.chunk_pages, pages);
-    const int share = (c_b - c_a + kWarps - 1) / kWarps;
-    const int a = c_a + warp * share, b = min(a + share, c_b);
-    const int32_t* table = p.tables + seq * p.table_stride;
-    bool bad = false;
+    const int most = len - nq + min(r0 + COLS - 1, nrows - 1) / p.group + 1, pages = pages_of_length(most);
     auto address = [&](int page) {
-        int block = __ldg(table + page / p.pages_per_block);
         if (block < 0 || block >= p.num_blocks) {
             bad = true;
             block = block < 0 ? 0 : static_cast<int>(p.num_blocks - 1);
         }
         return page_address<D>(p, page, block, kvh);
     };
-    if (a < b) {
-        Page<D> x;
-        const uint8_t* base = address(a);
+    Page<D> x;
+    if (first < pages) {
+        const uint8_t* base = address(first);
         load_keys<D>(x, base, lane);
         load_values<D>(x, base, lane);
-        for (int page = a; page < b; ++page) {
-            const bool more = page + 1 < b;
-            const uint8_t* next = more ? address(page + 1) : nullptr;
-            float s[NT][4];
-            uint32_t weights[NT][2];
-            page_scores<D, NT>(s, w, x);
-            const float2 scales = x.scales;
-            if (more) load_keys<D>(x, next, lane);
-            page_weights<D, NT>(w, s, scales, page, weights);
-            page_products<D, NT>(w, x, weights, page, lane);
-            if (more) load_values<D>(x, next, lane);
+        block = ask(first + stride);
+    }
+    Rows<D, NT> w;
+    set_queries<D, NT, BF16>(w, words, p, r0, nrows, len, nq, lane);
+#pragma unroll 1
+    for (int page = first; page < pages; page += stride) {
+        const bool more = page + stride < pages;
+        const uint8_t* next = more ? address(page + stride) : nullptr;
+        float s[NT][4];
+        uint32_t weights[NT][2];
+        page_scores<D, NT>(s, w, x);
+        const float2 scales = x.scales;
+        if (more) load_keys<D>(x, next, lane);
+        page_weights<D, NT>(w, s, scales, page, weights);
+        page_products<D, NT>(w, x, weights, page, lane);
+        if (more) {
+            load_values<D>(x, next, lane);
+            block = ask(page + 2 * stride);
         }
     }
     if (bad && p.status) atomicOr(p.status, TQ_STATUS_BAD_BLOCK);
@@ -411,45 +471,85 @@ __global__ void __launch_bounds__(kWarps * 32) attend8_kernel(const Attend8Param
             for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             const int col = 8 * n + 2 * t + j;
             const float up = ex2(w.u[n][j] - w.m[n][j] - kHeadroom);
+            float* at = part_o + (warp * COLS + col) * D + D / 8 * g;
 #pragma unroll
-            for (int i = 0; i < Rows<D, NT>::kSteps; ++i) {
-                part_o[warp][col][D / 8 * g + 2 * i] = w.o[i][n][j] * up;
-                part_o[warp][col][D / 8 * g + 2 * i + 1] = w.o[i][n][j + 2] * up;
-            }
-            if (g == 0) {
-                part_m[warp][col] = w.m[n][j];
-                part_l[warp][col] = l;
-            }
+            for (int i = 0; i < D / 16; i += 2)
+                *reinterpret_cast<float4*>(at + 2 * i) =
+                    make_float4(w.o[i][n][j] * up, w.o[i][n][j + 2] * up, w.o[i + 1][n][j] * up, w.o[i + 1][n][j + 2] * up);
+            if (g == 0) *reinterpret_cast<float2*>(part_s + (warp * COLS + col) * 2) = make_float2(w.m[n][j], l);
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * NT * D; i += kWarps * 32) {
-        const int col = i / D, d = i % D, row = r0 + col;
-        if (row >= nrows) break;
-        float m = kNothing, l = 0.f, o = 0.f;
+    // A warp joins the parts of one row at a time: lane k < WARPS knows warp k's statistics, a lane sums D / 32 dims.
+    for (int col = warp; col < COLS; col += WARPS) {
+        const int row = r0 + col;
+        const float2 stat = lane < WARPS ? *reinterpret_cast<const float2*>(part_s + (lane * COLS + col) * 2) : make_float2(kNothing, 0.f);
+        float m = stat.x;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) m = fmaxf(m, part_m[k][col]);
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float f = ex2(stat.x - m);
+        float l = f * stat.y;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-            const float f = ex2(part_m[k][col] - m);
-            l += f * part_l[k][col];
-            o += f * part_o[k][col][d];
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float o[D / 32] = {};
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float* at = part_o + (k * COLS + col) * D + lane * (D / 32);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) o[i] += fk * at[i];
         }
-        const int token = row / p.group, head = kvh * p.group + row - token * p.group;
-        const int64_t at = static_cast<int64_t>(first_row + token) * p.q_heads + head;
-        if (p.chunks == 1 || chunks == 1) {
-            store_out(p.out, at * D + d, l == 0.f ? 0.f : o / l, BF16);
+        if (p.chunks == 1) {
+            if (row < nrows) store_row<D, BF16>(p, first_row, kvh, row, o, l, lane);
         } else {
-            float* to = p.partials + (at * p.chunks + chunk) * (D + 2);
-            to[d] = o;
-            if (d == 0) {
-                to[D] = m;
-                to[D + 1] = l;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) own_o[col * D + lane * (D / 32) + i] = o[i];
+            if (lane == 0) {
+                own_s[col * 2] = m;
+                own_s[col * 2 + 1] = l;
             }
         }
     }
+    if (p.chunks == 1) return;
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // Rows are dealt out to the CTAs; lane k knows CTA k's statistics.
+    for (int col = part + p.chunks * warp; col < COLS; col += p.chunks * WARPS) {
+        const int row = r0 + col;
+        if (row >= nrows) continue;
+        float2 stat = load_cluster2(cluster_address(smem_u32(own_s + col * 2), lane < p.chunks ? lane : 0));
+        float from[kMaxCluster][D / 32];
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            const uint32_t at = cluster_address(smem_u32(own_o + col * D + lane * (D / 32)), k < p.chunks ? k : 0);
+#pragma unroll
+            for (int i = 0; i < D / 32; i += 2) {
+                const float2 x2 = load_cluster2(at + 4 * i);
+                from[k][i] = x2.x;
+                from[k][i + 1] = x2.y;
+            }
+        }
+        if (lane >= p.chunks) stat = make_float2(kNothing, 0.f);
+        float m = stat.x;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float f = lane < p.chunks ? ex2(stat.x - m) : 0.f;
+        float l = f * stat.y;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float o[D / 32] = {};
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            if (k < p.chunks) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] += fk * from[k][i];
+            }
+        }
+        store_row<D, BF16>(p, first_row, kvh, row, o, l, lane);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody's memory is read any more
 }
 
-// One warp per query row joins the parts of its chunks.
+// One warp per query row joins the parts of prompt attention whose keys were shared out.
 template <int D>
 __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params p, int bf16) {
     pdl_release();
@@ -459,21 +559,13 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params 
     int first_row, nq;
     rows_of(p, seq, first_row, nq);
     if (r >= nq * p.q_heads) return;
-    const int token = r / p.q_heads, head = r - token * p.q_heads, kvh = head / p.group, row = token * p.group + head - kvh * p.group;
-    const int len = min(p.seq_lens[seq], p.max_pages * kPageTokens);
-    int chunks = p.chunks;                              // prompt chunks: every part is written
-    if (p.chunk_pages) {
-        const int last = min(row / p.tile_rows * p.tile_rows + p.tile_rows - 1, nq * p.group - 1);
-        const int pages = pages_of_length(len - nq + last / p.group + 1);
-        chunks = (pages + p.chunk_pages - 1) / p.chunk_pages;
-        if (chunks <= 1) return;                     // written by its only chunk
-    }
+    const int token = r / p.q_heads, head = r - token * p.q_heads;
     const int64_t at = static_cast<int64_t>(first_row + token) * p.q_heads + head;
     const float* part = p.partials + at * p.chunks * (D + 2);
     float m = kNothing;
-    for (int c = 0; c < chunks; ++c) m = fmaxf(m, part[c * (D + 2) + D]);
+    for (int c = 0; c < p.chunks; ++c) m = fmaxf(m, part[c * (D + 2) + D]);
     float l = 0.f, o[D / 32] = {};
-    for (int c = 0; c < chunks; ++c) {
+    for (int c = 0; c < p.chunks; ++c) {
         const float f = ex2(part[c * (D + 2) + D] - m);
         l += f * part[c * (D + 2) + D + 1];
 #pragma unroll
@@ -492,11 +584,11 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params 
 namespace tq {
 namespace {
 
-enum class Attend8Kind { kChunks, kStream, kPrompt };
+enum class Attend8Kind { kFew, kStream, kPrompt };
 
 struct Attend8Plan {
     Attend8Kind kind;
-    int nt, tiles, chunk_pages, chunks;
+    int nt, warps, tiles, chunks;       // warps of a CTA and CTAs of a cluster (kFew), parts of an item's keys (kPrompt)
 };
 
 // Which kernel, and how it is cut.
@@ -516,15 +608,13 @@ Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries,
     a.tiles = static_cast<int>((rows + 8 * a.nt - 1) / (8 * a.nt));
     const int64_t items = seqs * kv_heads * a.tiles;
     // The persistent kernel needs a page or two per warp of the GPU at least.
-    a.kind = items * max_pages >= 4736 ? Attend8Kind::kStream : Attend8Kind::kChunks;
-    int64_t want = (148 * 4 + items - 1) / items;                       // chunks per item that fill the GPU
-    const int64_t most = (max_pages + 15) / 16;
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    a.chunk_pages = static_cast<int>((max_pages + want - 1) / want);
-    if (a.chunk_pages < 1) a.chunk_pages = 1;
-    a.chunks = (max_pages + a.chunk_pages - 1) / a.chunk_pages;
-    if (a.chunks < 1) a.chunks = 1;
+    a.kind = items * max_pages >= 32768 ? Attend8Kind::kStream : Attend8Kind::kFew;
+    // One CTA of 16 warps (8 for 16 query rows) fits an SM, or four of 4.
+    a.warps = items > kMaxCtas ? 4 : a.nt == 1 ? 16 : 8;
+    a.chunks = 1;
+    // Clusters lie within a part of the GPU: 35 of 4 CTAs and 16 of 8 fit next to one another, and a margin is left (16 of 8: 20.6 us, 16 of 4: 13).
+    const int64_t fit[] = {0, 148, 74, 0, 32, 0, 0, 0, 12};
+    while (a.chunks < kMaxCluster && items <= fit[a.chunks * 2] && a.chunks * a.warps < max_pages) a.chunks *= 2;
     return a;
 }
 
@@ -532,7 +622,7 @@ int64_t attend8_workspace(const Attend8Plan& a, int64_t rows, int q_heads, int h
     if (a.kind == Attend8Kind::kStream)
         return 4 * (head_dim == 64 ? (a.nt == 1 ? StreamSpace<64, 1>::kFloats : StreamSpace<64, 2>::kFloats)
                                    : (a.nt == 1 ? StreamSpace<128, 1>::kFloats : StreamSpace<128, 2>::kFloats));
-    return a.chunks == 1 ? 0 : rows * q_heads * a.chunks * (head_dim + 2) * 4;
+    return a.kind == Attend8Kind::kFew || a.chunks == 1 ? 0 : rows * q_heads * a.chunks * (head_dim + 2) * 4;
 }
 
 // The opt-in shared-memory size is a per-device function attribute; set once per device.
@@ -552,13 +642,33 @@ cudaError_t launch_merge(const Attend8Params& p, bool bf16, cudaStream_t stream)
     return launch_chained(attend8_merge_kernel<D>, dim3(static_cast<unsigned>(p.merge_blocks) * p.seqs), dim3(128), 0, stream, p, static_cast<int>(bf16));
 }
 
+template <int D, int NT, bool BF16, int WARPS>
+cudaError_t launch_few(const Attend8Params& p, cudaStream_t stream) {
+    static bool configured[64] = {};
+    auto kernel = attend8_few_kernel<D, NT, BF16, WARPS>;
+    constexpr int kSmem = few_smem(D, NT, WARPS);
+    const cudaError_t err = allow_shared_memory(kernel, kSmem, configured);
+    if (err != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.chunks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.chunks > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <int D, int NT, bool BF16>
-cudaError_t launch_rows(const Attend8Params& p, bool persistent, cudaStream_t stream) {
-    if (!persistent) {
-        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
-        const cudaError_t err = launch_chained(attend8_kernel<D, NT, BF16>, grid, dim3(kWarps * 32), 0, stream, p);
-        return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, BF16, stream);
-    }
+cudaError_t launch_rows(const Attend8Params& p, const Attend8Plan& a, cudaStream_t stream) {
+    if (a.kind == Attend8Kind::kFew)
+        return a.warps == 4 ? launch_few<D, NT, BF16, 4>(p, stream) : launch_few<D, NT, BF16, (NT == 1 ? 16 : 8)>(p, stream);
     static bool configured[64] = {};
     auto kernel = attend8_stream_kernel<D, NT, BF16>;
     cudaError_t err = allow_shared_memory(kernel, StreamSmem<D, NT>::kBytes, configured);
@@ -578,9 +688,8 @@ cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, bool bf
         err = launch_chained(attend8_prompt_kernel<D>, grid, dim3(kPromptThreads), PromptSmem<D>::kBytes, stream, p, static_cast<int>(bf16));
         return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, bf16, stream);
     }
-    const bool persistent = a.kind == Attend8Kind::kStream;
-    if (a.nt == 1) return bf16 ? launch_rows<D, 1, true>(p, persistent, stream) : launch_rows<D, 1, false>(p, persistent, stream);
-    return bf16 ? launch_rows<D, 2, true>(p, persistent, stream) : launch_rows<D, 2, false>(p, persistent, stream);
+    if (a.nt == 1) return bf16 ? launch_rows<D, 1, true>(p, a, stream) : launch_rows<D, 1, false>(p, a, stream);
+    return bf16 ? launch_rows<D, 2, true>(p, a, stream) : launch_rows<D, 2, false>(p, a, stream);
 }
 
 }  // namespace
@@ -630,7 +739,7 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     p.partials = static_cast<float*>(workspace); p.status = status; p.num_blocks = num_blocks; p.table_stride = bt_stride;
     p.scale_log2 = sm_scale * kLog2e; p.rows = static_cast<int>(num_rows); p.seqs = num_seqs; p.q_heads = num_q_heads; p.kv_heads = num_kv_heads;
     p.group = num_q_heads / num_kv_heads; p.pages_per_block = block_size / kPageTokens; p.max_pages = max_pages_per_seq; p.max_queries = max_queries;
-    p.tiles = a.tiles; p.tile_rows = 8 * a.nt; p.merge_blocks = static_cast<int>(merge_blocks); p.chunk_pages = a.chunk_pages; p.chunks = a.chunks; p.zero_tail = zero_tail;
+    p.tiles = a.tiles; p.merge_blocks = static_cast<int>(merge_blocks); p.chunks = a.chunks; p.zero_tail = zero_tail;
     const cudaError_t err = head_dim == 64 ? launch_attend8<64>(p, a, io_dtype == TQ_DTYPE_BF16, stream)
                                            : launch_attend8<128>(p, a, io_dtype == TQ_DTYPE_BF16, stream);
     return err == cudaSuccess ? TQ_OK : TQ_ERR_LAUNCH;

@@ -165,24 +165,6 @@ __device__ __forceinline__ void read_values(Page<D>& x, uint32_t stage, int lane
     }
 }
 
-__device__ __forceinline__ uint32_t pack_out(float a, float b, bool bf16) {
-    if (bf16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return pack_half2(a, b);
-}
-
-// A query row's output from its D / 32 sums of each lane.
-template <int D, bool BF16>
-__device__ __forceinline__ void store_row(const Attend8Params& p, const PartEntry& item, int row, const float (&o)[D / 32], float l, int lane) {
-    const int token = row / p.group, head = item.kvh * p.group + row - token * p.group;
-    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + (static_cast<int64_t>(item.first_row + token) * p.q_heads + head) * D) + lane * (D / 64);
-    const float f = 1.f / l;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) to[i] = l == 0.f ? 0u : pack_out(o[2 * i] * f, o[2 * i + 1] * f, BF16);
-}
-
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(stream_warps(NT) * 32, 1) attend8_stream_kernel(const Attend8Params p) {
     using Smem = StreamSmem<D, NT>;
@@ -436,7 +418,7 @@ __global__ void __launch_bounds__(stream_warps(NT) * 32, 1) attend8_stream_kerne
                 }
         }
         if (done) {
-            store_row<D, BF16>(p, head, row, o, l, lane);
+            store_row<D, BF16>(p, head.first_row, head.kvh, row, o, l, lane);
         } else {
             const int64_t at = static_cast<int64_t>(blockIdx.x) * 2 + (head.begins ? 1 : 0);
             float* to = p.partials + at * Space::kPart + col * D + lane * (D / 32);
@@ -541,7 +523,7 @@ __global__ void __launch_bounds__(256) attend8_stream_merge_kernel(const Attend8
     }
 #pragma unroll
     for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-    store_row<D, BF16>(p, head, head.r0 + col, o, l, lane);
+    store_row<D, BF16>(p, head.first_row, head.kvh, head.r0 + col, o, l, lane);
 }
 
 }  // namespace

@@ -123,6 +123,23 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& d
     return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
 }
 
+// Vectors that share one allocation: an allocation takes most of a small output's host time.
+struct Vectors {
+    at::Tensor bytes;
+    int64_t used = 0;
+    Vectors(int64_t total, const at::Device& dev) : bytes(empty({total}, at::kByte, dev)) {}
+    static int64_t room(int64_t n, int64_t item) { return (n * item + 15) / 16 * 16; }
+    at::Tensor take(int64_t n, at::ScalarType type) {
+        const int64_t item = c10::elementSize(type);
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(bytes.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                                c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(n);
+        t.unsafeGetTensorImpl()->set_storage_offset(used / item);
+        used += room(n, item);
+        return t;
+    }
+};
+
 tq_stream_t stream_of(const at::Device& dev) {
     return reinterpret_cast<tq_stream_t>(c10::cuda::getCurrentCUDAStream(dev.index()).stream());
 }
@@ -575,8 +592,9 @@ PyObject* plan_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         return declined();
     const at::Device dev = query.device();
     const c10::cuda::CUDAGuard guard(dev);
-    at::Tensor slots = empty({v[1]}, at::kLong, dev), positions = empty({v[1]}, at::kLong, dev), lens = empty({n}, at::kInt, dev);
-    at::Tensor starts = empty({n + 1}, at::kInt, dev), left = empty({1}, at::kInt, dev);
+    Vectors out(2 * Vectors::room(v[1], 8) + Vectors::room(n, 4) + Vectors::room(n + 1, 4) + 16, dev);
+    at::Tensor slots = out.take(v[1], at::kLong), positions = out.take(v[1], at::kLong), lens = out.take(n, at::kInt);
+    at::Tensor starts = out.take(n + 1, at::kInt), left = out.take(1, at::kInt);
     const tq_stream_t stream = stream_of(dev);
     const int rc = launch([&] {
         return L.plan_step(query.data_ptr<int32_t>(), context.data_ptr<int32_t>(), tables.data_ptr<int32_t>(), tables.stride(0),
@@ -605,7 +623,8 @@ PyObject* release_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         return declined();
     const at::Device dev = ended.device();
     const c10::cuda::CUDAGuard guard(dev);
-    at::Tensor lens = empty({n}, at::kInt, dev), left = empty({1}, at::kInt, dev);
+    Vectors out(Vectors::room(n, 4) + 16, dev);
+    at::Tensor lens = out.take(n, at::kInt), left = out.take(1, at::kInt);
     const tq_stream_t stream = stream_of(dev);
     const int rc = launch([&] {
         return L.release_blocks(reinterpret_cast<const uint8_t*>(ended.data_ptr<bool>()), context.data_ptr<int32_t>(), tables.data_ptr<int32_t>(),

@@ -51,6 +51,11 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t (&to
     b = before[1] + y - b;
 }
 
+// Blocks of n tokens: lengths fit 31 bits, and a 64-bit division takes a hundred instructions.
+__device__ __forceinline__ int blocks_of(int n, int block_size) {
+    return static_cast<int>((static_cast<uint32_t>(n) + static_cast<uint32_t>(block_size) - 1u) / static_cast<uint32_t>(block_size));
+}
+
 struct PlanParams {
     const int32_t* query_lens;
     const int32_t* context_lens;
@@ -94,9 +99,10 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanParams p) {
         }
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const int64_t total = (ctx[j] + query[j] + p.block_size - 1) / p.block_size;
-            wide[j] = total <= p.width && ctx[j] + query[j] <= INT32_MAX;
-            need[j] = wide[j] ? total - (ctx[j] + p.block_size - 1) / p.block_size : 0;
+            const int64_t tokens = ctx[j] + query[j];
+            const int total = tokens <= INT32_MAX ? blocks_of(static_cast<int>(tokens), p.block_size) : 0;
+            wide[j] = tokens <= INT32_MAX && total <= p.width;
+            need[j] = wide[j] ? total - blocks_of(static_cast<int>(ctx[j]), p.block_size) : 0;
             sum_rows += query[j];
             sum_need += need[j];
         }
@@ -140,8 +146,9 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanParams p) {
             const int64_t pos = static_cast<int64_t>(context[lo]) + (r - begin);
             int64_t slot = -1;
             if (first_free[lo] >= 0) {
-                const int at = static_cast<int>(pos / p.block_size), in_block = static_cast<int>(pos - static_cast<int64_t>(at) * p.block_size);
-                const int held = static_cast<int>((static_cast<int64_t>(context[lo]) + p.block_size - 1) / p.block_size);
+                // a request that is served ends before 2^31
+                const int at = static_cast<int>(static_cast<uint32_t>(pos) / static_cast<uint32_t>(p.block_size)), in_block = static_cast<int>(pos) - at * p.block_size;
+                const int held = blocks_of(context[lo], p.block_size);
                 int32_t* entry = p.tables + (c0 + lo) * p.table_stride + at;
                 int32_t block;
                 if (at >= held) {
@@ -209,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams p
             const int i = c0 + threadIdx.x * kPer + j;
             const bool ends = i < p.requests && p.ended[i];
             const int64_t ctx = i < p.requests ? p.context_lens[i] : 0;
-            give[j] = ends && ctx > 0 ? (ctx + p.block_size - 1) / p.block_size : 0;
+            give[j] = ends && ctx > 0 ? blocks_of(static_cast<int>(ctx), p.block_size) : 0;
             if (give[j] > p.width) {
                 give[j] = p.width;
                 flags |= TQ_STATUS_TOO_LONG;
@@ -231,9 +238,9 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams p
         for (int i = blockIdx.x * (kThreads / 32) + warp; i < n; i += gridDim.x * (kThreads / 32)) {
             const int32_t* from = p.tables + (c0 + i) * p.table_stride;
             const int64_t to = place[i];
-            for (int j = lane; j < held[i]; j += 32) {
-                if (to + j < p.free_size) p.free_blocks[to + j] = from[j];
-            }
+            const int n = static_cast<int>(min(static_cast<int64_t>(held[i]), p.free_size - to));
+#pragma unroll 4
+            for (int j = lane; j < n; j += 32) p.free_blocks[to + j] = __ldg(from + j);
         }
         __syncthreads();
     }

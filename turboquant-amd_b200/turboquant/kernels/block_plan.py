@@ -6,16 +6,16 @@ requests back.  Nothing comes back to the host, so a captured step can build its
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
 from turboquant.kernels import _native
 
 
-@dataclass
-class StepPlan:
-    """slot_mapping, positions: int64 [num_rows]; seq_lens: int32 [n]; query_start_loc: int32 [n + 1]; free_count: int32 [1]."""
+class StepPlan(NamedTuple):
+    """slot_mapping, positions: int64 [num_rows]; seq_lens: int32 [n]; query_start_loc: int32 [n + 1]; free_count: int32 [1].
+    They may lie in one allocation."""
 
     slot_mapping: torch.Tensor
     positions: torch.Tensor
@@ -38,9 +38,9 @@ def plan_step(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables
     if not torch.compiler.is_compiling():
         res = _native.host().plan_step(query_lens, context_lens, block_tables, free_blocks, free_count, block_size, num_rows)
         if res is not None:
-            return StepPlan(*res)
-    return StepPlan(*torch.ops.tq_b200.plan_step(query_lens, context_lens, block_tables, free_blocks, free_count, int(block_size),
-                                                 int(num_rows)))
+            return StepPlan._make(res)
+    return StepPlan._make(torch.ops.tq_b200.plan_step(query_lens, context_lens, block_tables, free_blocks, free_count, int(block_size),
+                                                     int(num_rows)))
 
 
 def release_blocks(ended: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, free_blocks: torch.Tensor,

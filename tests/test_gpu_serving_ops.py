@@ -343,6 +343,35 @@ def test_scores_of_any_size():
     _check_attention(gen(4), [300, 40], [1, 1], 8, 2, 128, 16, torch.bfloat16, q_size=1e-30, sm_scale=1e28)
 
 
+@pytest.mark.parametrize("width,n", [(0, 1), (9000, 1), (0, 40)])
+def test_values_of_very_different_sizes(width, n):
+    """Pages whose values are 2^24 apart: the small ones count for the denominator, whatever fp16 holds of their weights."""
+    for dtype, spread, scale in ((torch.float16, 9, 3e-5), (torch.bfloat16, 30, 2.0 ** -42)):
+        _check_attention(gen(n), [300, 140], [n, n], 8, 2, 128, 16, dtype, spread=spread, sm_scale=scale, width=width)
+
+
+@pytest.mark.parametrize("width,n", [(0, 1), (9000, 1), (0, 40)])
+def test_a_token_that_takes_all_is_exact(width, n):
+    """One key is the query's, the others are far: the output is that token's value, rounded once."""
+    g = gen(31)
+    H, D, bs, L = 2, 128, 16, 200
+    cache, tables = _filled(g, [L], H, D, bs)
+    codes, scales = codes_and_scales(cache, bs)
+    scales[..., 0] = 1.0
+    q = torch.zeros(n, 4 * H, D, device=DEV, dtype=torch.float16)
+    raw = codes.view(torch.uint8)
+    raw[:, :, :, 0] = 0                                                     # all keys zero but that of token 100, dim 7
+    b, at = int(tables[0, 100 // bs]), 100 % bs
+    raw[b, :, 0, 0, at, 7] = 0x7e
+    q[..., 7] = 30.0
+    if width:
+        tables = torch.nn.functional.pad(tables, (0, width - tables.shape[1]))
+    more = {} if n == 1 else dict(query_start_loc=torch.tensor([0, n], **i32), max_query_len=n)
+    got = paged_attention_8bit(q, cache, tables, torch.tensor([L], **i32), bs, sm_scale=1.0, **more)
+    want = (codes[b, :, 0, 1, at].float() * scales[b, :, 0, 1][:, None]).half()
+    assert torch.equal(got, want.repeat_interleave(4, 0).expand(n, -1, -1))
+
+
 def test_nan_reaches_what_sees_it_and_nothing_else():
     """A NaN value in a token that some queries of a chunk see and earlier ones do not; a NaN key."""
     g = gen(11)

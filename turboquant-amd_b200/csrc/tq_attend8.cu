@@ -27,6 +27,7 @@ struct Attend8Params {
 
 constexpr float kNothing = -3e38f;      // reference of a row that has seen no token: below every score, and finite, so that differences are numbers
 constexpr float kLazy = 8.f;            // a score may pass the reference by so much before it is raised
+constexpr float kSmallValues = 16.f;    // page_weights
 constexpr float kHeadroom = 6.f;        // weights are multiplied by 2^6: at most 2^14 in fp16, full precision down to 2^-20 of the largest
 
 // What one warp holds while it walks over pages of a sequence, for 8 * NT query rows against one KV head.
@@ -281,12 +282,20 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
     for (int n = 0; n < NT; ++n) {
         float e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            w.l[n][j & 1] += ex2(fmaf(s[n][j], c[n][j & 1], -w.m[n][j & 1]));
-            e[j] = ex2(fmaf(s[n][j], c[n][j & 1], ev + kHeadroom - w.u[n][j & 1]));
+        for (int j = 0; j < 4; ++j) e[j] = ex2(fmaf(s[n][j], c[n][j & 1], ev + kHeadroom - w.u[n][j & 1]));
+        // The denominator sums the weights as they are rounded for the product, so that a rounding common to both cancels: a token that takes
+        // nearly all is then exact.  Where the page's values are 2^16 below the reference, fp16 may not hold its weights, and they matter
+        // for the denominator alone.
+        const uint32_t lo = pack_half2(e[0], e[1]), hi = pack_half2(e[2], e[3]);
+        const float2 a = unpack_half2(lo), b = unpack_half2(hi);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float up = w.u[n][j] - ev - w.m[n][j];
+            const float sum = up > kSmallValues ? e[j] + e[j + 2] : j ? a.y + b.y : a.x + b.x;
+            w.l[n][j] = fmaf(sum, ex2(fminf(up - kHeadroom, 126.f)), w.l[n][j]);        // never infinite: zero times that would be NaN
         }
-        weights[n][0] = movmatrix_trans(pack_half2(e[0], e[1]));      // tokens 2t, 2t + 1 of column g
-        weights[n][1] = movmatrix_trans(pack_half2(e[2], e[3]));
+        weights[n][0] = movmatrix_trans(lo);        // tokens 2t, 2t + 1 of column g
+        weights[n][1] = movmatrix_trans(hi);
     }
 }
 
@@ -681,11 +690,13 @@ cudaError_t launch_rows(const Attend8Params& p, const Attend8Plan& a, cudaStream
 template <int D>
 cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, bool bf16, cudaStream_t stream) {
     if (a.kind == Attend8Kind::kPrompt) {
-        static bool configured[64] = {};
-        cudaError_t err = allow_shared_memory(attend8_prompt_kernel<D>, PromptSmem<D>::kBytes, configured);
+        static bool known[2][64] = {};
+        auto kernel = bf16 ? attend8_prompt_kernel<D, true> : attend8_prompt_kernel<D, false>;
+        bool(&configured)[64] = known[bf16];
+        cudaError_t err = allow_shared_memory(kernel, PromptSmem<D>::kBytes, configured);
         if (err != cudaSuccess) return err;
         const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
-        err = launch_chained(attend8_prompt_kernel<D>, grid, dim3(kPromptThreads), PromptSmem<D>::kBytes, stream, p, static_cast<int>(bf16));
+        err = launch_chained(kernel, grid, dim3(kPromptThreads), PromptSmem<D>::kBytes, stream, p);
         return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, bf16, stream);
     }
     if (a.nt == 1) return bf16 ? launch_rows<D, 1, true>(p, a, stream) : launch_rows<D, 1, false>(p, a, stream);

@@ -376,9 +376,9 @@ __device__ __forceinline__ float exchange(float* row, int half, int barrier, flo
     return theirs;
 }
 
-template <int D>
+template <int D, bool BF16>
 __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int split, uint8_t* smem, uint64_t* bars, volatile int* flags, uint32_t tmem,
-                               bool bf16, float row_scale) {
+                               float row_scale) {
     using Smem = PromptSmem<D>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = warp >> 3, half = warp >> 2 & 1, together = q * 4 + (warp & 3);
     const int row = job.r0 + q * kTile + (warp & 3) * 32 + lane;
@@ -430,12 +430,27 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
                     unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
                     y = ex2(y);
                     z = ex2(z);
-                    sums = add2(sums, pair(y, z));
                     w[8 * g + i] = pack_half2(y, z);
+                    if (!BF16) {
+                        // as they are rounded for the product (page_weights); an output in bf16 does not show the difference
+                        const float2 v = unpack_half2(w[8 * g + i]);
+                        y = v.x;
+                        z = v.y;
+                    }
+                    sums = add2(sums, pair(y, z));
+                }
+                if (!BF16 && __any_sync(0xffffffffu, u - ev - m > kSmallValues)) {
+                    sums = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float y, z;
+                        unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
+                        sums = add2(sums, pair(ex2(y), ex2(z)));
+                    }
                 }
                 float sum0, sum1;
                 unpair(sums, sum0, sum1);
-                sum = fmaf(sum0 + sum1, ex2(-shift - m), sum);               // in units of m again
+                sum = fmaf(sum0 + sum1, ex2(fminf(-shift - m, 126.f)), sum); // in units of m again; pages that are not there have v_exp -127
             }
             if (again) break;
             // Both warps of the rows decide alike, also about giving up.
@@ -514,7 +529,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
             for (int i = 0; i < 2; ++i) {
                 uint32_t v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = pack_out(__uint_as_float(x[8 * i + 2 * j]), __uint_as_float(x[8 * i + 2 * j + 1]), bf16);
+                for (int j = 0; j < 4; ++j) v[j] = pack_out(__uint_as_float(x[8 * i + 2 * j]), __uint_as_float(x[8 * i + 2 * j + 1]), BF16);
                 to[i] = make_uint4(v[0], v[1], v[2], v[3]);
             }
         } else {
@@ -528,8 +543,8 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
 
 // Queries of a tile as K-major A operand, two threads a row; returns the factor of its scores in units of log2.  All threads of the block
 // come here (a row's largest value is looked for by both of its threads), those of no row with row = -1.
-template <int D>
-__device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, uint8_t* smem, bool bf16) {
+template <int D, bool BF16>
+__device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, uint8_t* smem) {
     using Smem = PromptSmem<D>;
     constexpr int kWords = D / 4;
     const int warp = threadIdx.x >> 5, q = warp >> 3, half = warp >> 2 & 1, r = threadIdx.x & (kTile - 1), row = job.r0 + q * kTile + r;
@@ -550,7 +565,7 @@ __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, ui
 #pragma unroll
         for (int i = 0; i < kWords; ++i) x[i] = 0;
     }
-    if (bf16) {      // into the range of fp16 by a power of two, as in load_queries
+    if constexpr (BF16) {      // into the range of fp16 by a power of two, as in load_queries
 #pragma unroll
         for (int i = 0; i < kWords; ++i) most = max(most, max(x[i] & 0x7fffu, x[i] >> 16 & 0x7fffu));
         if (mine) largest[threadIdx.x] = most;
@@ -560,7 +575,7 @@ __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, ui
     }
     if (!mine) return 0.f;
     float row_scale = fabsf(p.scale_log2);
-    if (bf16) {
+    if constexpr (BF16) {
         const int e = min(max(static_cast<int>(most >> 7) - 127, -120), 120);
         const float down = exp2_int(-e);
 #pragma unroll
@@ -574,8 +589,8 @@ __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, ui
     return row_scale;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const Attend8Params p, int bf16) {
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const Attend8Params p) {
     using Smem = PromptSmem<D>;
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
@@ -637,14 +652,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem) + Smem::kTmemSlot), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const float row_scale = prompt_queries<D>(p, job, smem, bf16 != 0);
+    const float row_scale = prompt_queries<D, BF16>(p, job, smem);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     prompt_fence_before();
     __syncthreads();
     prompt_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Smem::kTmemSlot);
     if (warp < kSoftmaxWarps) {
-        if (warp < 8 * job.tiles) prompt_softmax<D>(p, job, split, smem, bars, flags, tmem, bf16 != 0, row_scale);
+        if (warp < 8 * job.tiles) prompt_softmax<D, BF16>(p, job, split, smem, bars, flags, tmem, row_scale);
     } else if (warp < kSoftmaxWarps + 2) {
         prompt_convert<D, false>(job, smem, bars, flags);
     } else if (warp < kSoftmaxWarps + 4) {

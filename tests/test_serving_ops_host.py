@@ -159,8 +159,8 @@ def test_cache8_calls_refuse_without_touching_a_gpu():
     assert attend(q=NULL) == attend(tables=NULL) == attend(blocks=0) == attend(hq=7) == attend(most=0) == attend(T=1) == attend(most=2) == -1
     assert attend(q=at(8)) == attend(out=at(8)) == attend(cache=at(8)) == -1
     assert attend(dtype=2) == attend(D=96) == attend(bs=8) == attend(pages=(1 << 27)) == -2
-    assert attend(T=1, ns=1, pages=8192) == -4                             # shared out over the GPU, and no workspace
-    need = L.tq_attend8_workspace_bytes(1, 1, 8, 2, 128, 1, 8192)
+    assert attend(T=1, ns=1, pages=20000) == -4                             # shared out over the GPU, and no workspace
+    need = L.tq_attend8_workspace_bytes(1, 1, 8, 2, 128, 1, 20000)
     assert need > 0 and L.tq_attend8_workspace_bytes(0, 0, 8, 2, 128, 1, 256) == 0
     assert L.tq_attend8_workspace_bytes(1, 1, 8, 3, 128, 1, 256) == -1 and L.tq_attend8_workspace_bytes(1, 1, 8, 2, 96, 1, 256) == -2
 
@@ -203,3 +203,15 @@ def test_plan_of_the_oracle_by_hand():
     assert count == 1 and status == 0 and tables.tolist() == [[9, 13, 9], [9, 12, 9], [11, 9, 9]]
     lens, count, free = S.release([True, False, True], [5, 5, 3], tables, [10, 0, 0, 0, 0], 1, 4)
     assert lens.tolist() == [0, 5, 0] and count == 4 and free.tolist() == [10, 9, 13, 11, 0]
+
+
+# ---- the engine's hook ---------------------------------------------------------------------------------
+def test_eight_bit_backend():
+    pytest.importorskip("vllm")
+    from turboquant.integration import tq_b200_backend as B
+    backend = B.TurboQuantB200EightBitBackend
+    assert backend.get_impl_cls() is B.TurboQuantB200EightBitImpl and backend.get_supported_head_sizes() == [64, 128]
+    assert backend.get_kv_cache_shape(5, 32, 2, 128) == (5, 2, 2 * 4128) and backend.get_name() == "CUSTOM"
+    assert B.TurboQuantB200Backend.get_impl_cls() is B.TurboQuantB200Impl
+    with pytest.raises(NotImplementedError):
+        B.TurboQuantB200EightBitImpl(8, 128, 1.0, 2, sliding_window=64)

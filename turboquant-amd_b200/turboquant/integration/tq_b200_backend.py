@@ -11,6 +11,10 @@ prefill runs ordinary attention on the raw K/V of the step.  Differences:
   * the cache tensor is uint8 [num_blocks, num_kv_heads, block_size/16 * page_bytes]
     (TurboQuant packed pages), not FP4 nibbles plus side buffers of scales.
 
+A second backend, TurboQuantB200EightBitBackend, keeps a layer's keys and values in 8 bits (paged_8bit): for the protected boundary
+layers, which the packed cache leaves out, and for steps that continue cached context with several tokens, which it serves like
+any other (the reference's extend branch, tq_fp4_backend.py:555-601).
+
 The classes are built on first use so that importing this module does not import vLLM.
 Status: written against vLLM 0.22's v1 interface.  `do_kv_cache_update` and `forward` are exercised
 on a GPU with hand-built layer and metadata objects (decode, fresh prefill and steps that mix both);
@@ -26,7 +30,9 @@ import torch
 
 from turboquant.integration.vllm_backend import TurboQuantConfig, get_tq_config, turbo_compress_and_scatter
 from turboquant.kernels.paged import CacheFormat, paged_decode_attention
+from turboquant.kernels.paged_8bit import cache_shape_8bit, page_bytes_8bit, paged_attention_8bit, quantize_and_scatter
 
+EIGHT_BIT_BACKEND_PATH = "turboquant.integration.tq_b200_backend.TurboQuantB200EightBitBackend"
 BACKEND_PATH = "turboquant.integration.tq_b200_backend.TurboQuantB200Backend"
 _FORMATS = {"turbo2": CacheFormat(2, 2, True), "turbo3": CacheFormat(3, 3, True), "turbo4": CacheFormat(4, 4, False)}
 
@@ -106,8 +112,8 @@ def _build_classes():
                 self._layer_idx = digits[0] if digits else 0
             state = self.config.get_state(self._layer_idx, device)
             if state is None:
-                raise NotImplementedError(
-                    "protected boundary layers keep the engine's own KV cache; give them another backend")
+                raise NotImplementedError("protected boundary layers keep the engine's own KV cache; give them another backend "
+                                          "(TurboQuantB200EightBitBackend, or the engine's)")
             return state
 
         def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping):
@@ -194,19 +200,75 @@ def _build_classes():
                                cache_dtype_str: str = "auto"):
             return kv_cache_shape(num_blocks, block_size, num_kv_heads, head_size)
 
-    _classes = (TurboQuantB200Backend, TurboQuantB200Impl)
+    class TurboQuantB200EightBitImpl(AttentionImpl):
+        """A layer whose cache holds e4m3 codes with a scale per 16 tokens and head.  Decodes, fresh prompts and chunks that continue cached
+        context are one call over the cache, which the step's own tokens are already in."""
+
+        def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
+                     alibi_slopes: Optional[list] = None, sliding_window: Optional[int] = None,
+                     kv_cache_dtype: str = "auto", logits_soft_cap: Optional[float] = None,
+                     attn_type: str = AttentionType.DECODER, kv_sharing_target_layer_name: Optional[str] = None,
+                     **_ignored) -> None:
+            if alibi_slopes is not None or sliding_window is not None or logits_soft_cap is not None:
+                raise NotImplementedError("TurboQuant B200 backend: no ALiBi, sliding window or soft cap")
+            if attn_type != AttentionType.DECODER:
+                raise NotImplementedError("TurboQuant B200 backend: decoder self-attention only")
+            self.num_heads, self.head_size, self.scale, self.num_kv_heads = num_heads, head_size, float(scale), num_kv_heads
+            self.kv_cache_dtype = "turboquant"
+
+        def _block_size(self, kv_cache) -> int:
+            return kv_cache.shape[2] // page_bytes_8bit(self.head_size) * 16
+
+        def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping):
+            n = key.shape[0]
+            quantize_and_scatter(key.view(n, self.num_kv_heads, self.head_size), value.view(n, self.num_kv_heads, self.head_size), kv_cache,
+                                 slot_mapping[:n], self._block_size(kv_cache))
+
+        def forward(self, layer, query, key, value, kv_cache, attn_metadata, output=None, output_scale=None,
+                    output_block_scale=None):
+            assert output is not None, "accept_output_buffer: the engine provides the output tensor"
+            if output_scale is not None or output_block_scale is not None:
+                raise NotImplementedError("fused output quantisation is not supported")
+            if attn_metadata is None:
+                return output.fill_(0)
+            n = attn_metadata.num_actual_tokens
+            most = int(attn_metadata.max_query_len)
+            more = {} if most == 1 else dict(query_start_loc=attn_metadata.query_start_loc, max_query_len=most)
+            res = paged_attention_8bit(query[:n].view(n, self.num_heads, self.head_size), kv_cache, attn_metadata.block_table,
+                                       attn_metadata.seq_lens, self._block_size(kv_cache), sm_scale=self.scale,
+                                       max_seq_len=int(getattr(attn_metadata, "max_seq_len", 0) or 0), **more)
+            output[:n].view(n, self.num_heads, self.head_size).copy_(res)
+            return output
+
+        def fused_rope_kvcache_supported(self):
+            return False
+
+    class TurboQuantB200EightBitBackend(TurboQuantB200Backend):
+        @staticmethod
+        def get_impl_cls():
+            return TurboQuantB200EightBitImpl
+
+        @classmethod
+        def get_supported_head_sizes(cls):
+            return [64, 128]
+
+        @staticmethod
+        def get_kv_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_size: int,
+                               cache_dtype_str: str = "auto"):
+            return cache_shape_8bit(num_blocks, block_size, num_kv_heads, head_size)
+
+    _classes = {c.__name__: c for c in (TurboQuantB200Backend, TurboQuantB200Impl, TurboQuantB200EightBitBackend,
+                                        TurboQuantB200EightBitImpl)}
     return _classes
 
 
 def __getattr__(name: str):
-    if name == "TurboQuantB200Backend":
-        return _build_classes()[0]
-    if name == "TurboQuantB200Impl":
-        return _build_classes()[1]
+    if name in ("TurboQuantB200Backend", "TurboQuantB200Impl", "TurboQuantB200EightBitBackend", "TurboQuantB200EightBitImpl"):
+        return _build_classes()[name]
     raise AttributeError(name)
 
 
-def register() -> None:
-    """Make `--attention-backend CUSTOM` (AttentionBackendEnum.CUSTOM) resolve to this backend."""
+def register(eight_bit: bool = False) -> None:
+    """Make `--attention-backend CUSTOM` (AttentionBackendEnum.CUSTOM) resolve to this backend, or to the 8-bit one."""
     from vllm.v1.attention.backends.registry import AttentionBackendEnum, register_backend
-    register_backend(AttentionBackendEnum.CUSTOM, BACKEND_PATH)
+    register_backend(AttentionBackendEnum.CUSTOM, EIGHT_BIT_BACKEND_PATH if eight_bit else BACKEND_PATH)

@@ -26,6 +26,8 @@
 // All waits are bounded; one that gives up sets TQ_STATUS_TIMEOUT, every role leaves its loop and the tensor memory is freed.
 #pragma once
 
+#include <type_traits>
+
 namespace tq {
 namespace {
 
@@ -406,52 +408,57 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
         uint32_t w[32];
         for (bool again = false;; again = true) {
             float most = kNothing, most_v = kNothing;
-            sum = 0.f;
-            uint32_t x[2][16];
-            prompt_ld16(s_at, x[0]);
+            // Twice, so that the code for columns that see nothing does not lie in the way of the steps that have none.
+            auto pass = [&](auto cut) {
+                sum = 0.f;
+                uint32_t x[2][16];
+                prompt_ld16(s_at, x[0]);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                uint32_t(&of)[16] = x[g & 1];
-                prompt_wait_ld();
-                if (g < 3) prompt_ld16(s_at + 16 * g + 16, x[(g + 1) & 1]);
-                if (masked) hide(of, visible - 16 * g);
-                const float c = fmaxf(row_scale * plan.k_scale[4 * half + g], kTiny), ev = plan.v_exp[4 * half + g], shift = ev + kHeadroom - u;
-                float a = fmaxf(fmaxf(__uint_as_float(of[0]), __uint_as_float(of[1])), __uint_as_float(of[2]));
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t(&of)[16] = x[g & 1];
+                    prompt_wait_ld();
+                    if (g < 3) prompt_ld16(s_at + 16 * g + 16, x[(g + 1) & 1]);
+                    if constexpr (decltype(cut)::value) hide(of, visible - 16 * g);
+                    const float c = fmaxf(row_scale * plan.k_scale[4 * half + g], kTiny), ev = plan.v_exp[4 * half + g], shift = ev + kHeadroom - u;
+                    float a = fmaxf(fmaxf(__uint_as_float(of[0]), __uint_as_float(of[1])), __uint_as_float(of[2]));
 #pragma unroll
-                for (int i = 3; i < 15; i += 2) a = fmaxf(fmaxf(a, __uint_as_float(of[i])), __uint_as_float(of[i + 1]));
-                a = fmaxf(a, __uint_as_float(of[15])) * c;
-                most = fmaxf(most, a);
-                most_v = fmaxf(most_v, a + ev);
-                const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
-                uint64_t sums = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float y, z;
-                    unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
-                    y = ex2(y);
-                    z = ex2(z);
-                    w[8 * g + i] = pack_half2(y, z);
-                    if (!BF16) {
-                        // as they are rounded for the product (page_weights); an output in bf16 does not show the difference
-                        const float2 v = unpack_half2(w[8 * g + i]);
-                        y = v.x;
-                        z = v.y;
-                    }
-                    sums = add2(sums, pair(y, z));
-                }
-                if (!BF16 && __any_sync(0xffffffffu, u - ev - m > kSmallValues)) {
-                    sums = 0;
+                    for (int i = 3; i < 15; i += 2) a = fmaxf(fmaxf(a, __uint_as_float(of[i])), __uint_as_float(of[i + 1]));
+                    a = fmaxf(a, __uint_as_float(of[15])) * c;
+                    most = fmaxf(most, a);
+                    most_v = fmaxf(most_v, a + ev);
+                    const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
+                    uint64_t sums = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float y, z;
                         unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
-                        sums = add2(sums, pair(ex2(y), ex2(z)));
+                        y = ex2(y);
+                        z = ex2(z);
+                        w[8 * g + i] = pack_half2(y, z);
+                        if (!BF16) {
+                            // as they are rounded for the product (page_weights); an output in bf16 does not show the difference
+                            const float2 v = unpack_half2(w[8 * g + i]);
+                            y = v.x;
+                            z = v.y;
+                        }
+                        sums = add2(sums, pair(y, z));
                     }
+                    if (!BF16 && __any_sync(0xffffffffu, u - ev - m > kSmallValues)) {
+                        sums = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float y, z;
+                            unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
+                            sums = add2(sums, pair(ex2(y), ex2(z)));
+                        }
+                    }
+                    float sum0, sum1;
+                    unpair(sums, sum0, sum1);
+                    sum = fmaf(sum0 + sum1, ex2(fminf(-shift - m, 126.f)), sum); // in units of m again; pages that are not there have v_exp -127
                 }
-                float sum0, sum1;
-                unpair(sums, sum0, sum1);
-                sum = fmaf(sum0 + sum1, ex2(fminf(-shift - m, 126.f)), sum); // in units of m again; pages that are not there have v_exp -127
-            }
+            };
+            if (masked) pass(std::true_type{});
+            else pass(std::false_type{});
             if (again) break;
             // Both warps of the rows decide alike, also about giving up.
             const int mine = __any_sync(0xffffffffu, most > m + kLazy || most_v > u + kLazy) ? 1 : 0;
@@ -475,11 +482,12 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
                 prompt_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < D / 32; ++h) {
-                    prompt_ld16(o_at + 16 * h, x[0]);
+                    uint32_t o[16];
+                    prompt_ld16(o_at + 16 * h, o);
                     prompt_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * down);
-                    prompt_st16(o_at + 16 * h, x[0]);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
+                    prompt_st16(o_at + 16 * h, o);
                 }
             }
         }

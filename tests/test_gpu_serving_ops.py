@@ -329,6 +329,50 @@ def test_wide_tables_several_queries(D, Hq, H, bs):
     _check_attention(gen(Hq), lens, queries, Hq, H, D, bs, torch.bfloat16, width=4000)
 
 
+# Decodes, verified tokens and chunks in one call over many pages: two kernels share the sequences, by their number of query rows.
+_MIXED = [1, 1, 0, 4, 130, 1, 2, 16, 17, 1, 5, 64, 1, 3, 1, 8, 1, 0, 33, 1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,Hq,H,bs", [(128, 8, 2, 16), (64, 16, 1, 32), (128, 3, 3, 48), (128, 12, 1, 16), (64, 34, 2, 16), (64, 8, 8, 16)])
+def test_mixed_steps(D, Hq, H, bs, dtype):
+    g = gen(Hq + H)
+    lens = [n + int(x) for n, x in zip(_MIXED, torch.randint(0, 400, (len(_MIXED),), generator=torch.Generator().manual_seed(Hq)))]
+    lens[0], lens[5], lens[8], lens[13] = 0, 1, 17, 2                       # no context, nothing at all, fewer tokens than queries
+    _check_attention(g, lens, _MIXED, Hq, H, D, bs, dtype, width=40000 // (len(lens) * H * (bs // 16)) + 60)
+
+
+@pytest.mark.parametrize("n", [2, 128, 129, 705, 1500])
+def test_mixed_steps_of_many_sequences(n):
+    """One chunk among decodes, at either end or inside; more sequences than are ranked, and than a CTA has threads."""
+    for at in (0, n // 2, n - 1):
+        queries, lens = [1] * n, [1 + (37 * i + at) % 70 for i in range(n)]
+        queries[at], lens[at] = 150, 333
+        _check_attention(gen(n), lens, queries, 8, 2, 64, 16, torch.bfloat16, width=40000 // (2 * n) + 60)
+
+
+def test_mixed_steps_with_chunks_that_fill_the_gpu():
+    _check_attention(gen(3), [40, 900, 33, 1000, 2, 0, 650], [1, 610, 2, 1, 2, 1, 40], 32, 8, 128, 16, torch.float16, width=700)
+
+
+@pytest.mark.parametrize("width", [4, 2000])
+def test_rows_behind_a_mixed_step(width):
+    g = gen(21)
+    queries, lens = [1, 70, 0, 1, 3], [50, 100, 20, 1, 33]
+    q, cache, tables, lens_t, got = _check_attention(g, lens, queries, 8, 4, 128, 16, torch.float16, width=width)
+    padded = torch.cat([q, torch.randn(9, 8, 128, generator=g, device=DEV).half()])
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(queries)]), **i32)
+    new = paged_attention_8bit(padded, cache, tables, lens_t, 16, query_start_loc=starts, max_query_len=70)
+    out = torch.full_like(padded, 7.0)
+    paged_attention_8bit(padded, cache, tables, lens_t, 16, query_start_loc=starts, max_query_len=70, out=out)
+    assert torch.equal(new[:75], out[:75]) and not new[75:].any() and (out[75:] == 7).all()
+    assert torch.equal(new[:75], got)                                       # rows behind change nothing
+    paged_attention_8bit(padded, cache, tables, lens_t, 16, query_start_loc=starts, max_query_len=65)
+    assert _native.read_status(DEV) == _native.STATUS_TOO_LONG
+    paged_attention_8bit(padded, cache, tables, lens_t + 16 * 3 * 2000, 16, query_start_loc=starts, max_query_len=70)
+    assert _native.read_status(DEV) & _native.STATUS_BAD_BLOCK
+
+
 def test_negative_and_zero_scales():
     for width in (0, 9000):
         _check_attention(gen(5), [300, 40], [1, 1], 8, 2, 128, 16, torch.float16, sm_scale=-0.05, width=width)

@@ -22,7 +22,8 @@ struct Attend8Params {
     int32_t* status;
     int64_t num_blocks, table_stride;
     float scale_log2;
-    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, chunks, merge_blocks, zero_tail;
+    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, chunks, zero_tail;
+    int small_rows;                 // not 0: sequences of at most so many query rows have one kernel, the others another one
 };
 
 constexpr float kNothing = -3e38f;      // reference of a row that has seen no token: below every score, and finite, so that differences are numbers
@@ -564,12 +565,19 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const Attend8Params 
     pdl_release();
     pdl_wait();
     const int lane = threadIdx.x & 31;
-    const int seq = blockIdx.x / p.merge_blocks, r = (blockIdx.x - seq * p.merge_blocks) * 4 + (threadIdx.x >> 5);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (at >= static_cast<int64_t>(p.rows) * p.q_heads) return;
+    const int row = static_cast<int>(at / p.q_heads);
+    int seq = p.starts ? 0 : row, end = p.seqs;                     // the last sequence that begins at or before the row
+    while (p.starts && end - seq > 1) {
+        const int mid = (seq + end) >> 1;
+        if (p.starts[mid] <= row) seq = mid;
+        else end = mid;
+    }
+    if (seq >= p.seqs) return;
     int first_row, nq;
     rows_of(p, seq, first_row, nq);
-    if (r >= nq * p.q_heads) return;
-    const int token = r / p.q_heads, head = r - token * p.q_heads;
-    const int64_t at = static_cast<int64_t>(first_row + token) * p.q_heads + head;
+    if (row < first_row || row - first_row >= nq || nq * p.group <= p.small_rows) return;
     const float* part = p.partials + at * p.chunks * (D + 2);
     float m = kNothing;
     for (int c = 0; c < p.chunks; ++c) m = fmaxf(m, part[c * (D + 2) + D]);
@@ -597,27 +605,43 @@ enum class Attend8Kind { kFew, kStream, kPrompt };
 
 struct Attend8Plan {
     Attend8Kind kind;
-    int nt, warps, tiles, chunks;       // warps of a CTA and CTAs of a cluster (kFew), parts of an item's keys (kPrompt)
+    int nt, warps, chunks;              // warps of a CTA and CTAs of a cluster (kFew), parts of an item's keys (kPrompt)
+    int64_t tiles;                      // of a sequence; of all sequences for kPrompt
+    int small_rows;                     // kPrompt: sequences of at most so many rows are left to the persistent kernel
 };
 
+// The persistent kernel needs a page or two per warp of the GPU at least.  (8 KV heads, 64 sequences of 512 tokens: 22.3 us, 16.0 in
+// clusters; 64 of 1024: 36.4, 31.9; one of 65536: 37.6, 54.7.)
+constexpr int64_t kStreamPages = 32768;
+
 // Which kernel, and how it is cut.
-Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
+Attend8Plan attend8_plan(int64_t num_rows, int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
     Attend8Plan a = {};
     const int64_t rows = static_cast<int64_t>(group) * max_queries;
     if (rows > 32) {
         a.kind = Attend8Kind::kPrompt;
-        a.tiles = static_cast<int>((rows + 2 * kTile - 1) / (2 * kTile));
-        const int64_t items = seqs * kv_heads * a.tiles, steps = (max_pages + 2 * kTilePages - 1) / (2 * kTilePages);
+        a.tiles = (rows + 2 * kTile - 1) / (2 * kTile) * seqs;
+        const int64_t full = num_rows * group / (2 * kTile);
+        if (full + seqs < a.tiles) a.tiles = full + seqs;
+        int64_t items = a.tiles;
+        // Decodes next to a chunk: a tile of 256 rows with 4 or 8 in use costs what a full one does.  (32 / 8 heads, 64 decodes over 8192 tokens and a
+        // chunk of 2048: 599 us, 1222 by one kernel; 200 over 1024 and two of 1024: 205, 639; 8 over 4096 and four of 512: 275, 288.)
+        if (group <= 16 && num_rows < seqs * max_queries && seqs * kv_heads * max_pages >= kStreamPages) {
+            a.small_rows = 16;
+            a.nt = group <= 8 ? 1 : 2;
+            items = full + 1;
+        }
+        items *= kv_heads;
+        const int64_t steps = (max_pages + 2 * kTilePages - 1) / (2 * kTilePages);
         int64_t want = kMaxCtas / items;                                // parts per item, of two steps at least, that fill the GPU
         if (want > steps) want = steps;
         a.chunks = static_cast<int>(want < 1 ? 1 : want);
         return a;
     }
     a.nt = rows <= 8 ? 1 : 2;
-    a.tiles = static_cast<int>((rows + 8 * a.nt - 1) / (8 * a.nt));
+    a.tiles = (rows + 8 * a.nt - 1) / (8 * a.nt);
     const int64_t items = seqs * kv_heads * a.tiles;
-    // The persistent kernel needs a page or two per warp of the GPU at least.
-    a.kind = items * max_pages >= 32768 ? Attend8Kind::kStream : Attend8Kind::kFew;
+    a.kind = items * max_pages >= kStreamPages ? Attend8Kind::kStream : Attend8Kind::kFew;
     // One CTA of 16 warps (8 for 16 query rows) fits an SM, or four of 4.
     a.warps = items > kMaxCtas ? 4 : a.nt == 1 ? 16 : 8;
     a.chunks = 1;
@@ -628,10 +652,15 @@ Attend8Plan attend8_plan(int64_t seqs, int kv_heads, int group, int max_queries,
 }
 
 int64_t attend8_workspace(const Attend8Plan& a, int64_t rows, int q_heads, int head_dim) {
-    if (a.kind == Attend8Kind::kStream)
-        return 4 * (head_dim == 64 ? (a.nt == 1 ? StreamSpace<64, 1>::kFloats : StreamSpace<64, 2>::kFloats)
+    int64_t need = 0;
+    if (a.kind == Attend8Kind::kStream || a.small_rows)
+        need = 4 * (head_dim == 64 ? (a.nt == 1 ? StreamSpace<64, 1>::kFloats : StreamSpace<64, 2>::kFloats)
                                    : (a.nt == 1 ? StreamSpace<128, 1>::kFloats : StreamSpace<128, 2>::kFloats));
-    return a.kind == Attend8Kind::kFew || a.chunks == 1 ? 0 : rows * q_heads * a.chunks * (head_dim + 2) * 4;
+    if (a.kind == Attend8Kind::kPrompt && a.chunks > 1) {                 // after the persistent kernel, in the same place
+        const int64_t parts = rows * q_heads * a.chunks * (head_dim + 2) * 4;
+        if (parts > need) need = parts;
+    }
+    return need;
 }
 
 // The opt-in shared-memory size is a per-device function attribute; set once per device.
@@ -648,7 +677,7 @@ cudaError_t allow_shared_memory(Kernel kernel, int bytes, bool (&configured)[64]
 
 template <int D>
 cudaError_t launch_merge(const Attend8Params& p, bool bf16, cudaStream_t stream) {
-    return launch_chained(attend8_merge_kernel<D>, dim3(static_cast<unsigned>(p.merge_blocks) * p.seqs), dim3(128), 0, stream, p, static_cast<int>(bf16));
+    return launch_chained(attend8_merge_kernel<D>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.rows) * p.q_heads + 3) / 4)), dim3(128), 0, stream, p, static_cast<int>(bf16));
 }
 
 template <int D, int NT, bool BF16, int WARPS>
@@ -675,9 +704,7 @@ cudaError_t launch_few(const Attend8Params& p, cudaStream_t stream) {
 }
 
 template <int D, int NT, bool BF16>
-cudaError_t launch_rows(const Attend8Params& p, const Attend8Plan& a, cudaStream_t stream) {
-    if (a.kind == Attend8Kind::kFew)
-        return a.warps == 4 ? launch_few<D, NT, BF16, 4>(p, stream) : launch_few<D, NT, BF16, (NT == 1 ? 16 : 8)>(p, stream);
+cudaError_t launch_stream(const Attend8Params& p, cudaStream_t stream) {
     static bool configured[64] = {};
     auto kernel = attend8_stream_kernel<D, NT, BF16>;
     cudaError_t err = allow_shared_memory(kernel, StreamSmem<D, NT>::kBytes, configured);
@@ -687,20 +714,30 @@ cudaError_t launch_rows(const Attend8Params& p, const Attend8Plan& a, cudaStream
     return launch_chained(attend8_stream_merge_kernel<D, NT, BF16>, dim3(kMaxCtas - 1, NT), dim3(256), 0, stream, p);
 }
 
-template <int D>
-cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, bool bf16, cudaStream_t stream) {
-    if (a.kind == Attend8Kind::kPrompt) {
-        static bool known[2][64] = {};
-        auto kernel = bf16 ? attend8_prompt_kernel<D, true> : attend8_prompt_kernel<D, false>;
-        bool(&configured)[64] = known[bf16];
-        cudaError_t err = allow_shared_memory(kernel, PromptSmem<D>::kBytes, configured);
-        if (err != cudaSuccess) return err;
-        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads * p.seqs));
-        err = launch_chained(kernel, grid, dim3(kPromptThreads), PromptSmem<D>::kBytes, stream, p);
-        return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, bf16, stream);
+template <int D, bool BF16>
+cudaError_t launch_prompt(const Attend8Params& p, cudaStream_t stream) {
+    static bool configured[64] = {};
+    auto kernel = attend8_prompt_kernel<D, BF16>;
+    cudaError_t err = allow_shared_memory(kernel, PromptSmem<D>::kBytes, configured);
+    if (err != cudaSuccess) return err;
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.chunks) * p.tiles * p.kv_heads));
+    err = launch_chained(kernel, grid, dim3(kPromptThreads), PromptSmem<D>::kBytes, stream, p);
+    return err != cudaSuccess || p.chunks == 1 ? err : launch_merge<D>(p, BF16, stream);
+}
+
+template <int D, bool BF16>
+cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, cudaStream_t stream) {
+    if (a.kind == Attend8Kind::kFew) {
+        if (a.nt == 1) return a.warps == 4 ? launch_few<D, 1, BF16, 4>(p, stream) : launch_few<D, 1, BF16, 16>(p, stream);
+        return a.warps == 4 ? launch_few<D, 2, BF16, 4>(p, stream) : launch_few<D, 2, BF16, 8>(p, stream);
     }
-    if (a.nt == 1) return bf16 ? launch_rows<D, 1, true>(p, a, stream) : launch_rows<D, 1, false>(p, a, stream);
-    return bf16 ? launch_rows<D, 2, true>(p, a, stream) : launch_rows<D, 2, false>(p, a, stream);
+    if (a.kind == Attend8Kind::kStream || a.small_rows) {
+        Attend8Params q = p;
+        if (a.small_rows) q.zero_tail = 0;                              // the other kernel's
+        const cudaError_t err = a.nt == 1 ? launch_stream<D, 1, BF16>(q, stream) : launch_stream<D, 2, BF16>(q, stream);
+        if (err != cudaSuccess || a.kind == Attend8Kind::kStream) return err;
+    }
+    return launch_prompt<D, BF16>(p, stream);
 }
 
 }  // namespace
@@ -713,7 +750,7 @@ extern "C" int64_t tq_attend8_workspace_bytes(int64_t num_rows, int num_seqs, in
         return TQ_ERR_ARG;
     if (head_dim != 64 && head_dim != 128) return TQ_ERR_UNSUPPORTED;
     if (num_seqs == 0) return 0;
-    const Attend8Plan a = attend8_plan(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
+    const Attend8Plan a = attend8_plan(num_rows, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
     return attend8_workspace(a, num_rows, num_q_heads, head_dim);
 }
 
@@ -738,10 +775,10 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     if (!out || !q || !cache || !block_tables || !seq_lens || num_blocks == 0) return TQ_ERR_ARG;
     if (!query_start_loc && (num_rows < num_seqs || max_queries != 1)) return TQ_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) % 16) return TQ_ERR_ARG;
-    const Attend8Plan a = attend8_plan(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
-    const int64_t merge_blocks = (static_cast<int64_t>(max_queries) * num_q_heads + 3) / 4;
-    if (static_cast<double>(num_kv_heads) * a.tiles * a.chunks * num_seqs > INT32_MAX || static_cast<double>(merge_blocks) * num_seqs > INT32_MAX)
-        return TQ_ERR_UNSUPPORTED;
+    const Attend8Plan a = attend8_plan(num_rows, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_queries, max_pages_per_seq);
+    double grid = static_cast<double>(a.tiles) * num_kv_heads * a.chunks * (a.kind == Attend8Kind::kPrompt ? 1 : num_seqs);
+    if (a.kind == Attend8Kind::kPrompt && a.chunks > 1) grid = fmax(grid, static_cast<double>(num_rows) * num_q_heads / 4);
+    if (grid > INT32_MAX - 1) return TQ_ERR_UNSUPPORTED;
     const int64_t need = attend8_workspace(a, num_rows, num_q_heads, head_dim);
     if (need && (!workspace || workspace_bytes < need)) return TQ_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return TQ_ERR_ARG;
@@ -750,8 +787,9 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     p.partials = static_cast<float*>(workspace); p.status = status; p.num_blocks = num_blocks; p.table_stride = bt_stride;
     p.scale_log2 = sm_scale * kLog2e; p.rows = static_cast<int>(num_rows); p.seqs = num_seqs; p.q_heads = num_q_heads; p.kv_heads = num_kv_heads;
     p.group = num_q_heads / num_kv_heads; p.pages_per_block = block_size / kPageTokens; p.max_pages = max_pages_per_seq; p.max_queries = max_queries;
-    p.tiles = a.tiles; p.merge_blocks = static_cast<int>(merge_blocks); p.chunks = a.chunks; p.zero_tail = zero_tail;
-    const cudaError_t err = head_dim == 64 ? launch_attend8<64>(p, a, io_dtype == TQ_DTYPE_BF16, stream)
-                                           : launch_attend8<128>(p, a, io_dtype == TQ_DTYPE_BF16, stream);
+    p.tiles = static_cast<int>(a.tiles); p.chunks = a.chunks; p.zero_tail = zero_tail; p.small_rows = a.small_rows;
+    const bool bf16 = io_dtype == TQ_DTYPE_BF16;
+    const cudaError_t err = head_dim == 64 ? (bf16 ? launch_attend8<64, true>(p, a, stream) : launch_attend8<64, false>(p, a, stream))
+                                           : (bf16 ? launch_attend8<128, true>(p, a, stream) : launch_attend8<128, false>(p, a, stream));
     return err == cudaSuccess ? TQ_OK : TQ_ERR_LAUNCH;
 }

@@ -598,6 +598,60 @@ __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, ui
     return row_scale;
 }
 
+// The sequence and its block of 256 query rows that slot `slot` stands for, -1 when there are fewer.  Only blocks that exist get a slot, so
+// that a batch of decodes with one chunk does not launch a CTA for every block that a decode could have had.  CTAs start in the
+// order of the slots: a sequence's blocks from the last one, which sees the most, down, and the longest sequence first, so that
+// the last CTAs are short: 16 uneven sequences 316 us (362 unsorted), 4 chunks of 512 to 2048 tokens 441 (453).
+__device__ __forceinline__ void prompt_place(const Attend8Params& p, int slot, int* shared, int& seq, int& block) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto blocks_of = [&](int s) {
+        int first_row, nq;
+        rows_of(p, s, first_row, nq);
+        return nq * p.group <= p.small_rows ? 0 : (nq * p.group + 2 * kTile - 1) / (2 * kTile);
+    };
+    auto take = [&](int s, uint32_t place, int blocks) {
+        if (place >= static_cast<uint32_t>(blocks)) return;
+        shared[0] = s;
+        shared[1] = blocks - 1 - static_cast<int>(place);
+    };
+    if (tid == 0) shared[0] = -1;
+    if (p.seqs <= kRankedSeqs) {
+        int2* all = reinterpret_cast<int2*>(shared + 2);                    // lengths, blocks
+        const int2 mine = tid < p.seqs ? make_int2(p.seq_lens[tid], blocks_of(tid)) : make_int2(0, 0);
+        if (tid < p.seqs) all[tid] = mine;
+        __syncthreads();
+        if (mine.y) {
+            uint32_t before = 0;
+            for (int i = 0; i < p.seqs; ++i) before += all[i].x > mine.x || (all[i].x == mine.x && i < tid) ? all[i].y : 0;
+            take(tid, slot - before, mine.y);
+        }
+    } else {
+        const int each = (p.seqs + kPromptThreads - 1) / kPromptThreads, first = tid * each;
+        uint32_t sum = 0;
+        for (int s = first; s < min(first + each, p.seqs); ++s) sum += blocks_of(s);
+        uint32_t before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        if (lane == 31) shared[2 + warp] = before;
+        __syncthreads();
+        before -= sum;
+        for (int w = 0; w < warp; ++w) before += shared[2 + w];
+        for (int s = first; s < min(first + each, p.seqs); ++s) {
+            const int blocks = blocks_of(s);
+            take(s, slot - before, blocks);
+            before += blocks;
+        }
+    }
+    __syncthreads();
+    // By a shuffle, so that the compiler knows them to be the same for a warp (2048 tokens over 16384: 718 to 725 us, 731 without).
+    seq = __shfl_sync(0xffffffffu, shared[0], 0);
+    block = __shfl_sync(0xffffffffu, shared[1], 0);
+    __syncthreads();                                                        // before queries take this place
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const Attend8Params p) {
     using Smem = PromptSmem<D>;
@@ -630,43 +684,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
     pdl_wait();
     pdl_release();
 
-    // splits of one block of rows side by side, then the KV heads, then blocks of rows from the last one, which sees the most, down, then sequences
+    // Splits of one block of rows side by side, then the KV heads, then the blocks of rows.
     int rest = blockIdx.x;
     const int split = rest % p.chunks;
     rest /= p.chunks;
     PromptJob job;
     job.kvh = rest % p.kv_heads;
-    rest /= p.kv_heads;
-    // CTAs start in this order.  Where there are more than the GPU holds, the longest sequences come first, so that the last ones are short:
-    // 16 uneven sequences 316 us (362 with blocks of all sequences from the last down), 4 prompts of 512 to 2048 441 (453), even ones 414 (410).
-    const int block = p.tiles - 1 - rest % p.tiles;
-    int seq = rest / p.tiles;
-    if (gridDim.x > kMaxCtas && p.seqs > 1 && p.seqs <= kRankedSeqs) {
-        int* lens = reinterpret_cast<int*>(smem + Smem::kQ);
-        if (tid < p.seqs) lens[tid] = p.seq_lens[tid];
-        __syncthreads();
-        if (tid < p.seqs) {
-            int rank = 0;
-            for (int i = 0; i < p.seqs; ++i) rank += lens[i] > lens[tid] || (lens[i] == lens[tid] && i < tid);
-            if (rank == seq) lens[kRankedSeqs] = tid;
-        }
-        __syncthreads();
-        seq = lens[kRankedSeqs];
-        __syncthreads();                                                    // before queries take this place
-    }
+    int seq, block;
+    prompt_place(p, rest / p.kv_heads, reinterpret_cast<int*>(smem + Smem::kQ), seq, block);
     if (p.zero_tail && blockIdx.x == 0) {
         const int64_t row = static_cast<int64_t>(p.q_heads) * D, used = p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs;
         for (int64_t i = used * row + tid; i < p.rows * row; i += kPromptThreads) static_cast<uint16_t*>(p.out)[i] = 0;
     }
-    const bool too_many = rows_of(p, seq, job.first_row, job.nq);
+    if (p.status && blockIdx.x == 0) {
+        for (int s = tid; s < p.seqs; s += kPromptThreads) {
+            const bool too_many = rows_of(p, s, job.first_row, job.nq), too_long = pages_of_length(p.seq_lens[s]) > p.max_pages;
+            if (too_many || too_long) atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
+        }
+    }
+    if (seq < 0) return;
+    rows_of(p, seq, job.first_row, job.nq);
     job.nrows = job.nq * p.group;
     job.r0 = block * 2 * kTile;
     job.len = p.seq_lens[seq];
-    const bool too_long = pages_of_length(job.len) > p.max_pages;
-    if (too_long) job.len = p.max_pages * kPageTokens;
-    if ((too_long || too_many) && p.status && tid == 0 && split == 0 && block == 0 && job.kvh == 0)
-        atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
-    if (job.r0 >= job.nrows) return;
+    if (pages_of_length(job.len) > p.max_pages) job.len = p.max_pages * kPageTokens;
     job.tiles = job.nrows - job.r0 > kTile ? 2 : 1;
     const int most = max(job.len - job.nq + min(job.r0 + 2 * kTile - 1, job.nrows - 1) / p.group + 1, 0);
     const int steps = (most + kTile - 1) / kTile, each = (steps + p.chunks - 1) / p.chunks;

@@ -57,6 +57,7 @@ template <int NT>
 __device__ __forceinline__ SeqInfo seq_info(const Attend8Params& p, int seq) {
     SeqInfo s;
     rows_of(p, seq, s.first_row, s.nq);
+    if (p.small_rows && s.nq * p.group > p.small_rows) s.nq = 0;           // left to the kernel of prompt chunks
     s.len = p.seq_lens[seq];
     if (pages_of_length(s.len) > p.max_pages) s.len = p.max_pages * kPageTokens;
     s.tiles = (s.nq * p.group + 8 * NT - 1) / (8 * NT);

@@ -17,7 +17,13 @@
 // and SM, 2048 cycles a tile pair) next to the products (2048 cycles); conversion and bookkeeping share the issue slots with them.
 // Four roles run different code at the same time, and what they repeat has to fit the instruction cache: with everything unrolled (28 KB of
 // instructions a step) it missed in 28 % of the cases, the next level was at 77 % of its rate, and a step took 7000 cycles.
-// So loops stay loops here, and the codes go through shared memory instead of registers.
+// So loops stay loops here, the codes go through shared memory instead of registers, and steps without hidden columns have a
+// loop without masks (482 us with one for both).
+//
+// 32 / 8 heads of 128, bf16: 4 chunks of 700 to 1024 tokens over 1000 to 7168 440-456 us (653-679 TFLOP/s), one of 2048 over 16384 720
+// (812), one of 4096 over nothing 207 (663).  A step of two tiles takes about 4600 cycles, 2048 of them products: what is left is the chain
+// from scores to weights to products and back (one group of eight products by itself 960 to 1120 cycles, 512 of them at work).
+// One tile a CTA with two buffers for scores: 580 us, as the codes are then converted for half as many rows.
 //
 // The pages' scales enter with the weights, as two numbers for each 16 columns of the scores: weight = 2^(s c_page + shift_page), so that
 // fp16 weights use their range whatever the scales are (page_weights in tq_attend8.cu has the same two references m and u).
@@ -601,7 +607,7 @@ __device__ float prompt_queries(const Attend8Params& p, const PromptJob& job, ui
 // The sequence and its block of 256 query rows that slot `slot` stands for, -1 when there are fewer.  Only blocks that exist get a slot, so
 // that a batch of decodes with one chunk does not launch a CTA for every block that a decode could have had.  CTAs start in the
 // order of the slots: a sequence's blocks from the last one, which sees the most, down, and the longest sequence first, so that
-// the last CTAs are short: 16 uneven sequences 316 us (362 unsorted), 4 chunks of 512 to 2048 tokens 441 (453).
+// the last CTAs are short: 16 uneven sequences 316 us (362 unsorted), 4 chunks of 700 to 1024 tokens 441 (453).
 __device__ __forceinline__ void prompt_place(const Attend8Params& p, int slot, int* shared, int& seq, int& block) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto blocks_of = [&](int s) {

@@ -373,6 +373,40 @@ def test_rows_behind_a_mixed_step(width):
     assert _native.read_status(DEV) & _native.STATUS_BAD_BLOCK
 
 
+def test_a_captured_mixed_step_follows_its_lengths():
+    """Which kernel has which sequence is decided on the device: a replay with other lengths is that step's result.  Two graphs in turn, and a call
+    on another stream between them."""
+    g = gen(31)
+    lens = [300, 90, 200, 64, 150, 500]
+    cache, tables = _filled(g, lens, 2, 128, 16)
+    tables = torch.nn.functional.pad(tables, (0, 3000), value=-9)
+    q = torch.randn(120, 8, 128, generator=g, device=DEV).half()
+    lens_t, starts = torch.tensor(lens, **i32), torch.zeros(7, **i32)
+    call = dict(query_start_loc=starts, max_query_len=100)
+    steps = [[1, 1, 100, 1, 1, 16], [64, 1, 0, 17, 1, 1], [1, 1, 1, 1, 1, 1], [0, 100, 2, 0, 18, 0]]
+    cum = [torch.tensor(np.concatenate([[0], np.cumsum(s)]), **i32) for s in steps]
+    starts.copy_(cum[0])
+    paged_attention_8bit(q, cache, tables, lens_t, 16, **call)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_attention_8bit(q, cache, tables, lens_t, 16, **call))
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for c in cum:
+        starts.copy_(c)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = paged_attention_8bit(q, cache, tables, lens_t, 16, query_start_loc=c, max_query_len=100)
+        for graph, out in zip(graphs, outs):
+            out.fill_(3)
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+        torch.cuda.synchronize()
+
+
 def test_negative_and_zero_scales():
     for width in (0, 9000):
         _check_attention(gen(5), [300, 40], [1, 1], 8, 2, 128, 16, torch.float16, sm_scale=-0.05, width=width)

@@ -28,7 +28,7 @@ struct Attend8Params {
 
 constexpr float kNothing = -3e38f;      // reference of a row that has seen no token: below every score, and finite, so that differences are numbers
 constexpr float kLazy = 8.f;            // a score may pass the reference by so much before it is raised
-constexpr float kSmallValues = 16.f;    // page_weights
+constexpr float kFarApart = 64.f;       // value scales so many powers of two apart: page_weights
 constexpr float kHeadroom = 6.f;        // weights are multiplied by 2^6: at most 2^14 in fp16, full precision down to 2^-20 of the largest
 
 // What one warp holds while it walks over pages of a sequence, for 8 * NT query rows against one KV head.
@@ -233,6 +233,12 @@ __device__ __forceinline__ bool has_nan(const Page<D>& x, int from, int lane) {
     return __any_sync(0xffffffffu, found != 0);
 }
 
+// What a weight in units of the values' reference counts for in the denominator.  That is the weight as it was rounded for the product, so that a
+// rounding common to both cancels and a token that takes nearly all is exact.  But fp16 has no full precision below 2^-14 and nothing below 2^-25: where
+// the page's values are 2^up below the reference, that is every weight below 2^(up - 31) of the largest, and there may be many
+// of them.  Such a weight counts as it is.
+__device__ __forceinline__ float counted(float weight, float rounded) { return weight < 6.103515625e-5f ? weight : rounded; }
+
 // One page.  The softmax keeps two references per column: m for the denominators and u, which includes the value scale 2^ev of the page, for the
 // products, whose fp16 weights then use their range whatever the pages' scales are.  Both are raised only where a score passes
 // them by 2^8: most pages need one vote and no shuffles.
@@ -284,16 +290,18 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
         float e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = ex2(fmaf(s[n][j], c[n][j & 1], ev + kHeadroom - w.u[n][j & 1]));
-        // The denominator sums the weights as they are rounded for the product, so that a rounding common to both cancels: a token that takes
-        // nearly all is then exact.  Where the page's values are 2^16 below the reference, fp16 may not hold its weights, and they matter
-        // for the denominator alone.
         const uint32_t lo = pack_half2(e[0], e[1]), hi = pack_half2(e[2], e[3]);
         const float2 a = unpack_half2(lo), b = unpack_half2(hi);
+        const float rounded[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const float up = w.u[n][j] - ev - w.m[n][j];
-            const float sum = up > kSmallValues ? e[j] + e[j + 2] : j ? a.y + b.y : a.x + b.x;
-            w.l[n][j] = fmaf(sum, ex2(fminf(up - kHeadroom, 126.f)), w.l[n][j]);        // never infinite: zero times that would be NaN
+            float sum = counted(e[j], rounded[j]) + counted(e[j + 2], rounded[j + 2]), unit = ex2(up - kHeadroom);
+            if (up > kFarApart) {               // fp32 may not hold the weights in these units either
+                sum = ex2(fmaf(s[n][j], c[n][j], -w.m[n][j])) + ex2(fmaf(s[n][j + 2], c[n][j], -w.m[n][j]));
+                unit = 1.f;
+            }
+            w.l[n][j] = fmaf(sum, unit, w.l[n][j]);
         }
         weights[n][0] = movmatrix_trans(lo);        // tokens 2t, 2t + 1 of column g
         weights[n][1] = movmatrix_trans(hi);

@@ -202,7 +202,7 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         StepPlan& plan = plans[slot];
         if (lane < kTilePages) {
             plan.k_scale[mine] = scales.x;
-            plan.v_exp[mine] = static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127);
+            plan.v_exp[mine] = here ? static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127) : 0.f;
         }
         if (lane == 0) {
             plan.token0 = token0;
@@ -412,12 +412,14 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
         // Weights are computed against the references as they are, and the largest scores on the way.  Only where these pass the
         // references - always at first - the references are raised, and the scores, which are still there, gone through again.
         float sum;
+        bool far;
         uint32_t w[32];
         for (bool again = false;; again = true) {
             float most = kNothing, most_v = kNothing;
             // Twice, so that the code for columns that see nothing does not lie in the way of the steps that have none.
             auto pass = [&](auto cut) {
                 sum = 0.f;
+                far = false;
                 uint32_t x[2][16];
                 prompt_ld16(s_at, x[0]);
 #pragma unroll
@@ -443,25 +445,18 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
                         z = ex2(z);
                         w[8 * g + i] = pack_half2(y, z);
                         if (!BF16) {
-                            // as they are rounded for the product (page_weights); an output in bf16 does not show the difference
+                            // as page_weights does; an output in bf16 does not show the difference
                             const float2 v = unpack_half2(w[8 * g + i]);
-                            y = v.x;
-                            z = v.y;
+                            y = counted(y, v.x);
+                            z = counted(z, v.y);
                         }
                         sums = add2(sums, pair(y, z));
                     }
-                    if (!BF16 && __any_sync(0xffffffffu, u - ev - m > kSmallValues)) {
-                        sums = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float y, z;
-                            unpair(fma2(pair(__uint_as_float(of[2 * i]), __uint_as_float(of[2 * i + 1])), c2, shift2), y, z);
-                            sums = add2(sums, pair(ex2(y), ex2(z)));
-                        }
-                    }
                     float sum0, sum1;
                     unpair(sums, sum0, sum1);
-                    sum = fmaf(sum0 + sum1, ex2(fminf(-shift - m, 126.f)), sum); // in units of m again; pages that are not there have v_exp -127
+                    const float up = u - ev - m;                             // the sum in units of m again; page_weights
+                    far |= up > kFarApart;
+                    sum = fmaf(sum0 + sum1, up > kFarApart ? 0.f : ex2(up - kHeadroom), sum);
                 }
             };
             if (masked) pass(std::true_type{});
@@ -499,6 +494,21 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
             }
         }
         if (!ok) break;
+        if (__any_sync(0xffffffffu, far)) {
+            // Value scales so far apart that fp32 may not hold the weights in units of u: those columns are read again.
+#pragma unroll 1
+            for (int g = 0; g < 4; ++g) {
+                uint32_t of[16];
+                prompt_ld16(s_at + 16 * g, of);
+                prompt_wait_ld();
+                hide(of, visible - 16 * g);
+                const float c = fmaxf(row_scale * plan.k_scale[4 * half + g], kTiny);
+                float more = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) more += ex2(fmaf(__uint_as_float(of[i]), c, -m));
+                if (u - plan.v_exp[4 * half + g] - m > kFarApart) sum += more;
+            }
+        }
         l += sum;
         prompt_st32(s_at, w);
         prompt_wait_st();

@@ -57,3 +57,56 @@ def test_denominators_keep_small_weights_of_small_values(far, key, N, dtype, n, 
 def test_denominators_of_value_scales_as_far_apart_as_they_get(far, value, key, n, H, seqs, width):
     """Pages of zeros have the least scale, 2^-100: their weights count whatever the scale of the others is."""
     _one_token_and_many(far, key, 1024, torch.bfloat16, n, H, seqs, width, value)
+
+
+# ---- NaN -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,width", [(1, 0), (1, 20000), (4, 0), (4, 20000), (40, 0)])
+def test_nan_behind_a_vanishing_weight_reaches_the_output(n, width):
+    """Values that are NaN in tokens whose scores lie 160 nats below the largest one: zero times NaN is NaN, wherever the work is cut."""
+    D, bs, H, L = 128, 16, 2, 3000
+    cache = allocate_cache_8bit(L // bs + 1, bs, H, DEV, D)
+    codes, scales = codes_and_scales(cache, bs, D)
+    raw = codes.view(torch.uint8)
+    raw[:, :, :, 1] = torch.randint(0, 0x70, raw[:, :, :, 1].shape, generator=gen(3), device=DEV, dtype=torch.uint8)
+    scales.fill_(1.0)
+    codes[:, :, :, 0, :, 0] = torch.tensor(-160.0, device=DEV).to(torch.float8_e4m3fn)
+    raw[0, :, 0, 0, 3, 0] = 0                                               # token 3 takes all
+    dims = []
+    for page in (1, 3, 15, 20, 47, 100, 180):                               # one dim for each page: of the same warp, CTA, a following and a far one
+        raw[page, :, 0, 1, 7, page % D] = 0x7f
+        dims.append(page % D)
+    table = torch.arange(L // bs + 1, **i32)
+    tables = torch.nn.functional.pad(table, (0, max(0, width - len(table))))[None]
+    q = torch.zeros(n, 4 * H, D, device=DEV, dtype=torch.float16)
+    q[..., 0] = 1.0
+    more = {} if n == 1 else dict(query_start_loc=torch.tensor([0, n], **i32), max_query_len=n)
+    got = paged_attention_8bit(q, cache, tables, torch.tensor([L], **i32), bs, sm_scale=1.0, **more)
+    want = codes[0, :, 0, 1, 3].float().repeat_interleave(4, 0)
+    want[:, dims] = math.nan
+    assert torch.equal(got.isnan(), want.isnan().expand(n, -1, -1))
+    fine = ~want.isnan().expand(n, -1, -1)
+    assert torch.equal(got[fine], want.half().expand(n, -1, -1)[fine])
+
+
+@pytest.mark.parametrize("width", [0, 20000])
+@pytest.mark.parametrize("n,G", [(4, 2), (8, 1), (5, 4), (8, 4)])
+def test_nan_of_a_few_queries_reaches_what_sees_it_and_nothing_else(n, G, width):
+    """A NaN value that the later queries see and the earlier ones do not, and a NaN key, in the kernels for up to 32 rows."""
+    g = gen(n * G)
+    cache, tables = _filled(g, [60, 60], 1, 128, 16)
+    codes, _ = codes_and_scales(cache, 16)
+    raw = codes.view(torch.uint8)
+    t = 60 - n + 2                                                          # seen from query 2 on
+    raw[int(tables[0, t // 16]), 0, 0, 1, t % 16, 77] = 0xff
+    raw[int(tables[1, t // 16]), 0, 0, 0, t % 16, 3] = 0x7f
+    tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+    q = torch.randn(2 * n, G, 128, generator=g, device=DEV).half()
+    starts, lens = torch.tensor([0, n, 2 * n], **i32), torch.tensor([60, 60], **i32)
+    got = paged_attention_8bit(q, cache, tables, lens, 16, query_start_loc=starts, max_query_len=n)
+    c, s = _state(cache, 16, 128)
+    want, tol = S.attention(q.double().cpu().numpy(), c, s, tables.cpu().numpy(), [60, 60], [0, n, 2 * n], 16, 128 ** -0.5, EPS[torch.float16])
+    g64 = got.double().cpu().numpy()
+    assert np.array_equal(np.isnan(g64), np.isnan(want))
+    assert np.isnan(g64[2:n, :, 77]).all() and not np.isnan(g64[:2]).any() and np.isnan(g64[n + 2:]).all()
+    fine = ~np.isnan(want)
+    assert (np.abs(g64 - want)[fine] <= tol[fine]).all()

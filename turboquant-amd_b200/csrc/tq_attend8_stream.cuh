@@ -399,16 +399,17 @@ __global__ void __launch_bounds__(stream_warps(NT) * 32, 1) attend8_stream_kerne
         float l = member ? f * stat.y : 0.f;
 #pragma unroll
         for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        // Parts four at a time; those beyond the last one have weight zero and are the last one's.
+        // Parts four at a time; beyond the last one it is read again and left out.  A part whose weight is zero counts: a NaN in its values does.
         float o[D / 32] = {};
         const int offset = col * D + lane * (D / 32);
         for (uint32_t rest = members; rest;) {
             float part[4][D / 32], weight[4];
+            bool more[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int e = rest ? __ffs(rest) - 1 : e1;
                 weight[k] = __shfl_sync(0xffffffffu, f, e);
-                if (!rest) weight[k] = 0.f;
+                more[k] = rest != 0;
                 const float* at = reinterpret_cast<const float*>(smem + (e & 1 ? (e >> 1) * Smem::kRing : Smem::kFirst + (e >> 1) * Smem::kPart));
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) part[k][i] = at[offset + i];
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(stream_warps(NT) * 32, 1) attend8_stream_kerne
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (weight[k] != 0.f) {
+                if (more[k]) {
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) o[i] += weight[k] * part[k][i];
                 }
@@ -509,8 +510,8 @@ __global__ void __launch_bounds__(256) attend8_stream_merge_kernel(const Attend8
         if (base == cta) {
 #pragma unroll
             for (int i = 0; i < kEarly; ++i) {
-                const float fk = i < n ? __shfl_sync(0xffffffffu, f, i) : 0.f;
-                if (fk != 0.f) {
+                if (i < n) {
+                    const float fk = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
                     for (int d = 0; d < D / 32; ++d) o[d] += fk * early[i][d];
                 }

@@ -293,15 +293,17 @@ int64_t tq_attend8_workspace_bytes(int64_t num_rows, int num_seqs, int num_q_hea
  * included, are in the cache; query_start_loc = NULL: row i is sequence i's
  * only one.  Row j of n sees the first seq_lens[i] - n + j + 1 tokens; one that
  * sees none becomes zeros.  max_queries: at least the most rows of a sequence
- * (the ones beyond are left out and flagged).  Rows behind the last sequence
- * are left as they were, or become zeros when zero_tail.  block_tables,
+ * (the ones beyond are left out and flagged, the others served as if they were
+ * all).  Rows that are left out or that no sequence has - before the first one,
+ * behind the last one - are left as they were, or become zeros when zero_rest.
+ * block_tables,
  * bt_stride, seq_lens, max_pages_per_seq, workspace, status: as in
  * tq_decode_paged. */
 int tq_attend8_paged(void* out, const void* q, int io_dtype, const void* cache, int64_t num_blocks, int block_size,
                      const int32_t* block_tables, int64_t bt_stride, const int32_t* seq_lens, const int32_t* query_start_loc,
                      float sm_scale, void* workspace, int64_t workspace_bytes, int32_t* status, int64_t num_rows,
                      int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int max_queries,
-                     int max_pages_per_seq, int zero_tail, tq_stream_t stream);
+                     int max_pages_per_seq, int zero_rest, tq_stream_t stream);
 
 /* Step tables from the requests' lengths.  Request i has context_lens[i] tokens
  * in the cache, in the first ceil(context / block_size) blocks of row i of

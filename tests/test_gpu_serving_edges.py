@@ -110,3 +110,51 @@ def test_nan_of_a_few_queries_reaches_what_sees_it_and_nothing_else(n, G, width)
     assert np.isnan(g64[2:n, :, 77]).all() and not np.isnan(g64[:2]).any() and np.isnan(g64[n + 2:]).all()
     fine = ~np.isnan(want)
     assert (np.abs(g64 - want)[fine] <= tol[fine]).all()
+
+
+# ---- rows that no sequence has -----------------------------------------------------------------------------
+def _after_garbage(q, *args, **kw):
+    """The call, with the allocator's block for its result full of NaN."""
+    junk = [torch.full_like(q, math.nan) for _ in range(3)]
+    del junk
+    return paged_attention_8bit(q, *args, **kw)
+
+
+@pytest.mark.parametrize("queries,lens,G,most,width", [
+    ([2, 3, 5], [20, 30, 40], 2, 3, 0), ([2, 3, 5], [20, 30, 40], 2, 3, 9000), ([2, 9, 0, 10], [20, 30, 7, 40], 4, 8, 0),
+    ([2, 9, 0, 10], [20, 30, 7, 40], 4, 8, 9000), ([70, 1, 90], [70, 5, 300], 4, 66, 0), ([70, 1, 0, 90, 3], [70, 5, 4, 300, 30], 4, 66, 9000)])
+def test_rows_that_are_left_out_or_that_no_sequence_has_are_zeros(queries, lens, G, most, width):
+    """Rows before the first sequence, behind the last one and beyond max_query_len: zeros in a new result, left as they were in `out`."""
+    g = gen(sum(queries))
+    cache, tables = _filled(g, lens, 2, 128, 16)
+    tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+    ahead, behind, T = 3, 4, sum(queries)
+    q = torch.randn(ahead + T + behind, 2 * G, 128, generator=g, device=DEV).half()
+    lens_t = torch.tensor(lens, **i32)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(queries)]) + ahead, **i32)
+    got = _after_garbage(q, cache, tables, lens_t, 16, query_start_loc=starts, max_query_len=most)
+    assert _native.read_status(DEV) == _native.STATUS_TOO_LONG
+    out = torch.full_like(q, 7.0)
+    paged_attention_8bit(q, cache, tables, lens_t, 16, query_start_loc=starts, max_query_len=most, out=out)
+    assert _native.read_status(DEV) == _native.STATUS_TOO_LONG
+    c, s = _state(cache, 16, 128)
+    # a sequence that is cut is served as if its first rows were all of them
+    cut = [min(n, most) for n in queries]
+    served = torch.zeros(len(q), dtype=torch.bool, device=DEV)
+    for i, n in enumerate(cut):
+        a = int(starts[i])
+        served[a:a + n] = True
+        want, tol = S.attention(q[a:a + n].double().cpu().numpy(), c, s, tables[i:i + 1].cpu().numpy(), [lens[i]], [0, n], 16, 128 ** -0.5, EPS[torch.float16])
+        assert (np.abs(got[a:a + n].double().cpu().numpy() - want) <= tol).all()
+    assert not got[~served].any() and (out[~served] == 7).all() and torch.equal(got[served], out[served])
+
+
+def test_offsets_that_are_none_touch_nothing_else():
+    g = gen(17)
+    cache, tables = _filled(g, [64, 64, 64], 2, 128, 16)
+    q = torch.randn(3, 4, 128, generator=g, device=DEV).bfloat16()
+    wild = torch.tensor([2, -7, 1 << 30, 3], **i32)                         # sequence 1 is cut to the tensor's rows, the others have none
+    around = torch.full((9, 4, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    paged_attention_8bit(q, cache, tables, torch.tensor([64, 64, 64], **i32), 16, query_start_loc=wild, max_query_len=2, out=around[3:6])
+    assert _native.read_status(DEV) == _native.STATUS_TOO_LONG
+    assert (around[:3] == 7).all() and (around[5:] == 7).all() and torch.isfinite(around).all()

@@ -22,7 +22,7 @@ struct Attend8Params {
     int32_t* status;
     int64_t num_blocks, table_stride;
     float scale_log2;
-    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, chunks, zero_tail;
+    int rows, seqs, q_heads, kv_heads, group, pages_per_block, max_pages, max_queries, tiles, chunks, zero_rest;
     int small_rows;                 // not 0: sequences of at most so many query rows have one kernel, the others another one
 };
 
@@ -390,15 +390,30 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, float x, bool b
     else static_cast<__half*>(out)[at] = __float2half_rn(x);
 }
 
-// The rows of a sequence, inside the tensors whatever `starts` says; true when it has more than the launch is sized for, which are left out.
-__device__ __forceinline__ bool rows_of(const Attend8Params& p, int seq, int& first_row, int& nq) {
+// The rows of a sequence, inside the tensors whatever `starts` says; returns how many more it has than the launch is sized for, which are left out.
+__device__ __forceinline__ int rows_of(const Attend8Params& p, int seq, int& first_row, int& nq) {
     first_row = seq;
     nq = 1;
-    if (!p.starts) return false;
+    if (!p.starts) return 0;
     first_row = min(max(p.starts[seq], 0), p.rows);
     const int n = max(min(p.starts[seq + 1], p.rows) - first_row, 0);
     nq = min(n, p.max_queries);
-    return n > p.max_queries;
+    return n - nq;
+}
+
+// A block's threads write zeros to rows a .. b.
+template <int D>
+__device__ __forceinline__ void zero_rows(const Attend8Params& p, int a, int b) {
+    const int64_t row = static_cast<int64_t>(p.q_heads) * D / 8;
+    uint4* out = static_cast<uint4*>(p.out);
+    for (int64_t i = a * row + threadIdx.x; i < b * row; i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Rows before the first sequence and behind the last one.
+template <int D>
+__device__ __forceinline__ void zero_ends(const Attend8Params& p) {
+    if (p.starts) zero_rows<D>(p, 0, min(max(p.starts[0], 0), p.rows));
+    zero_rows<D>(p, p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs, p.rows);
 }
 
 // Launches of few pages: a cluster of CTAs for each item (sequence, KV head, tile of 8 NT query rows), pages dealt out to the warps in
@@ -429,21 +444,19 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 && NT == 1 ? 4 : 1) att
     bool bad = false;
     auto ask = [&](int page) { return page < p.max_pages ? __ldg(table + page / p.pages_per_block) : 0; };
     int block = ask(first);
-    if (p.zero_tail && blockIdx.x == 0) {
-        const int64_t row = static_cast<int64_t>(p.q_heads) * D, used = p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs;
-        for (int64_t i = used * row + tid; i < p.rows * row; i += WARPS * 32) static_cast<uint16_t*>(p.out)[i] = 0;
-    }
+    if (p.zero_rest && blockIdx.x == 0) zero_ends<D>(p);
     int first_row, nq;
-    const bool too_many = rows_of(p, seq, first_row, nq);
+    const int left_out = rows_of(p, seq, first_row, nq);
     const int nrows = nq * p.group, r0 = tile * COLS;
     if (r0 >= nrows) return;                                        // the whole cluster
+    if (left_out && p.zero_rest && part == 0 && tile == 0 && kvh == 0) zero_rows<D>(p, first_row + nq, first_row + nq + left_out);
     int len = p.seq_lens[seq];
     QueryWords<D, NT> words;
     ask_queries<D, NT>(words, p, first_row, kvh, r0, nrows, lane);
     const bool too_long = pages_of_length(len) > p.max_pages;
     if (too_long) len = p.max_pages * kPageTokens;
-    if ((too_long || too_many) && p.status && tid == 0 && part == 0 && tile == 0 && kvh == 0)
-        atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
+    if ((too_long || left_out) && p.status && tid == 0 && part == 0 && tile == 0 && kvh == 0)
+        atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (left_out ? TQ_STATUS_TOO_LONG : 0));
     const int most = len - nq + min(r0 + COLS - 1, nrows - 1) / p.group + 1, pages = pages_of_length(most);
     auto address = [&](int page) {
         if (block < 0 || block >= p.num_blocks) {
@@ -742,7 +755,7 @@ cudaError_t launch_attend8(const Attend8Params& p, const Attend8Plan& a, cudaStr
     }
     if (a.kind == Attend8Kind::kStream || a.small_rows) {
         Attend8Params q = p;
-        if (a.small_rows) q.zero_tail = 0;                              // the other kernel's
+        if (a.small_rows) q.zero_rest = 0;                              // the other kernel's
         const cudaError_t err = a.nt == 1 ? launch_stream<D, 1, BF16>(q, stream) : launch_stream<D, 2, BF16>(q, stream);
         if (err != cudaSuccess || a.kind == Attend8Kind::kStream) return err;
     }
@@ -766,7 +779,7 @@ extern "C" int64_t tq_attend8_workspace_bytes(int64_t num_rows, int num_seqs, in
 extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const void* cache, int64_t num_blocks, int block_size,
                                 const int32_t* block_tables, int64_t bt_stride, const int32_t* seq_lens, const int32_t* query_start_loc,
                                 float sm_scale, void* workspace, int64_t workspace_bytes, int32_t* status, int64_t num_rows, int num_seqs,
-                                int num_q_heads, int num_kv_heads, int head_dim, int max_queries, int max_pages_per_seq, int zero_tail,
+                                int num_q_heads, int num_kv_heads, int head_dim, int max_queries, int max_pages_per_seq, int zero_rest,
                                 tq_stream_t stream) {
     using namespace tq;
     if (num_rows < 0 || num_seqs < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads || num_blocks < 0 || max_queries < 1 ||
@@ -777,7 +790,7 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     if (max_pages_per_seq > (1 << 26) || static_cast<int64_t>(max_queries) * num_q_heads > (1 << 30)) return TQ_ERR_UNSUPPORTED;
     if (num_rows == 0) return TQ_OK;
     if (num_seqs == 0) {
-        if (!zero_tail) return TQ_OK;
+        if (!zero_rest) return TQ_OK;
         if (!out) return TQ_ERR_ARG;
         return cudaMemsetAsync(out, 0, static_cast<size_t>(num_rows) * num_q_heads * head_dim * 2, stream) == cudaSuccess ? TQ_OK : TQ_ERR_LAUNCH;
     }
@@ -796,7 +809,7 @@ extern "C" int tq_attend8_paged(void* out, const void* q, int io_dtype, const vo
     p.partials = static_cast<float*>(workspace); p.status = status; p.num_blocks = num_blocks; p.table_stride = bt_stride;
     p.scale_log2 = sm_scale * kLog2e; p.rows = static_cast<int>(num_rows); p.seqs = num_seqs; p.q_heads = num_q_heads; p.kv_heads = num_kv_heads;
     p.group = num_q_heads / num_kv_heads; p.pages_per_block = block_size / kPageTokens; p.max_pages = max_pages_per_seq; p.max_queries = max_queries;
-    p.tiles = static_cast<int>(a.tiles); p.chunks = a.chunks; p.zero_tail = zero_tail; p.small_rows = a.small_rows;
+    p.tiles = static_cast<int>(a.tiles); p.chunks = a.chunks; p.zero_rest = zero_rest; p.small_rows = a.small_rows;
     const bool bf16 = io_dtype == TQ_DTYPE_BF16;
     const cudaError_t err = head_dim == 64 ? (bf16 ? launch_attend8<64, true>(p, a, stream) : launch_attend8<64, false>(p, a, stream))
                                            : (bf16 ? launch_attend8<128, true>(p, a, stream) : launch_attend8<128, false>(p, a, stream));

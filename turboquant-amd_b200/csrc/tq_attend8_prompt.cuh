@@ -708,18 +708,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
     job.kvh = rest % p.kv_heads;
     int seq, block;
     prompt_place(p, rest / p.kv_heads, reinterpret_cast<int*>(smem + Smem::kQ), seq, block);
-    if (p.zero_tail && blockIdx.x == 0) {
-        const int64_t row = static_cast<int64_t>(p.q_heads) * D, used = p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs;
-        for (int64_t i = used * row + tid; i < p.rows * row; i += kPromptThreads) static_cast<uint16_t*>(p.out)[i] = 0;
-    }
+    if (p.zero_rest && blockIdx.x == 0) zero_ends<D>(p);
     if (p.status && blockIdx.x == 0) {
         for (int s = tid; s < p.seqs; s += kPromptThreads) {
-            const bool too_many = rows_of(p, s, job.first_row, job.nq), too_long = pages_of_length(p.seq_lens[s]) > p.max_pages;
-            if (too_many || too_long) atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
+            const bool left_out = rows_of(p, s, job.first_row, job.nq) > 0, too_long = pages_of_length(p.seq_lens[s]) > p.max_pages;
+            if (left_out || too_long) atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (left_out ? TQ_STATUS_TOO_LONG : 0));
         }
     }
     if (seq < 0) return;
-    rows_of(p, seq, job.first_row, job.nq);
+    const int left_out = rows_of(p, seq, job.first_row, job.nq);
+    if (left_out && p.zero_rest && block == 0 && split == 0 && job.kvh == 0) zero_rows<D>(p, job.first_row + job.nq, job.first_row + job.nq + left_out);
     job.nrows = job.nq * p.group;
     job.r0 = block * 2 * kTile;
     job.len = p.seq_lens[seq];

@@ -447,20 +447,16 @@ __global__ void __launch_bounds__(stream_warps(NT) * 32, 1) attend8_stream_kerne
     }
 
     const int row_words = p.q_heads * D / 2;
-    if (p.zero_tail && blockIdx.x == 0) {
-        const int64_t used = p.starts ? min(max(p.starts[p.seqs], 0), p.rows) : p.seqs;
-        for (int64_t i = used * row_words + tid; i < static_cast<int64_t>(p.rows) * row_words; i += W * 32) static_cast<uint32_t*>(p.out)[i] = 0;
-    }
+    if (p.zero_rest && blockIdx.x == 0) zero_ends<D>(p);
     for (int s = blockIdx.x; s < p.seqs; s += gridDim.x) {
         const SeqInfo i = seq_info<NT>(p, s);
-        if (!i.pages) {
-            uint32_t* to = static_cast<uint32_t*>(p.out) + static_cast<int64_t>(i.first_row) * row_words;
-            for (int64_t k = tid; k < static_cast<int64_t>(i.nq) * row_words; k += W * 32) to[k] = 0;
-        }
+        if (!i.pages) zero_rows<D>(p, i.first_row, i.first_row + i.nq);
+        int first_row, nq;
+        const int left_out = rows_of(p, s, first_row, nq);
+        if (left_out && p.zero_rest) zero_rows<D>(p, first_row + nq, first_row + nq + left_out);
         if (tid == 0 && p.status) {
-            int first_row, nq;
-            const bool too_many = rows_of(p, s, first_row, nq), too_long = pages_of_length(p.seq_lens[s]) > p.max_pages;
-            if (too_many || too_long) atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (too_many ? TQ_STATUS_TOO_LONG : 0));
+            const bool too_long = pages_of_length(p.seq_lens[s]) > p.max_pages;
+            if (left_out || too_long) atomicOr(p.status, (too_long ? TQ_STATUS_BAD_BLOCK : 0) | (left_out ? TQ_STATUS_TOO_LONG : 0));
         }
     }
 }

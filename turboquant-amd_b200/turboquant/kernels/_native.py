@@ -417,7 +417,7 @@ def _check_cache8(cache: torch.Tensor, block_size: int, head_dim: int) -> None:
 
 
 def _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_scale: float, block_size: int, max_query_len: int,
-                  max_seq_len: int, zero_tail: bool) -> None:
+                  max_seq_len: int, zero_rest: bool) -> None:
     dev = _require_cuda(out, q, cache, block_tables, seq_lens, query_start_loc)
     if q.dim() != 3 or q.shape[-1] not in (64, 128) or not q.is_contiguous():
         raise ValueError("q must be contiguous [tokens, q_heads, 64 or 128]")
@@ -461,7 +461,7 @@ def _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_sca
         ws = workspace(dev, need)
         rc = L.tq_attend8_paged(_ptr(out), _ptr(q), _DTYPES[q.dtype], _ptr(cache), nb, block_size, _ptr(block_tables), block_tables.stride(0),
                                 _ptr(seq_lens), _ptr(query_start_loc), float(sm_scale), _ptr(ws), ws.numel(), _ptr(status_word(dev)), T, ns,
-                                Hq, Hkv, D, int(max_query_len), max_pages, int(zero_tail), _stream(dev))
+                                Hq, Hkv, D, int(max_query_len), max_pages, int(zero_rest), _stream(dev))
     _check(rc, "tq_attend8_paged")
 
 
@@ -587,7 +587,7 @@ def attend8_paged_op(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.T
                      query_start_loc: Optional[torch.Tensor], sm_scale: float, block_size: int, max_query_len: int,
                      max_seq_len: int) -> torch.Tensor:
     out = torch.empty_like(q)
-    _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_scale, block_size, max_query_len, max_seq_len, zero_tail=True)
+    _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_scale, block_size, max_query_len, max_seq_len, zero_rest=True)
     return out
 
 

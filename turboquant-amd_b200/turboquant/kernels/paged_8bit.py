@@ -73,8 +73,9 @@ def paged_attention_8bit(q: torch.Tensor, cache: torch.Tensor, block_tables: tor
     Without query_start_loc row i is the only query of sequence i.  With it (int32 [num_seqs + 1], ascending) rows
     query_start_loc[i] .. query_start_loc[i + 1] are the last tokens of sequence i, causal among themselves: row j of n sees
     the first seq_lens[i] - n + j + 1 tokens, and max_query_len is at least the largest n (rows beyond it are left out and
-    set STATUS_TOO_LONG).  The tokens themselves are in the cache already.  Rows that see nothing become zeros; rows behind
-    the last sequence become zeros too, or are left as they were when `out` is given.
+    set STATUS_TOO_LONG; the others are served as if they were all).  The tokens themselves are in the cache already.  Rows that
+    see nothing become zeros; rows that are left out or that no sequence has - before the first one, behind the last one - become
+    zeros too, or are left as they were when `out` is given.
     max_seq_len: the longest sequence of the step when the host knows it; launch and workspace are sized for it.
     sm_scale defaults to 1 / sqrt(D).  Query head h reads KV head h // (Hq // Hkv).
     """
@@ -97,5 +98,5 @@ def paged_attention_8bit(q: torch.Tensor, cache: torch.Tensor, block_tables: tor
     if torch.is_grad_enabled() and (q.requires_grad or out.requires_grad):
         raise RuntimeError("paged_attention_8bit(out=...) has no autograd")
     _native._attend8_impl(out, q.contiguous(), cache, block_tables, seq_lens.contiguous(), query_start_loc, sm_scale, block_size,
-                          max_query_len, max_seq_len, zero_tail=False)
+                          max_query_len, max_seq_len, zero_rest=False)
     return out

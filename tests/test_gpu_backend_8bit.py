@@ -48,3 +48,30 @@ def test_prompts_decodes_and_extends(D, Hq, H, bs, dtype):
             assert (got - want).norm() <= 0.08 * want.norm()
             a += new[i]
     assert _native.read_status(DEV) == 0
+
+
+@pytest.mark.parametrize("new", [(0, 1, 1, 0, 1), (1, 0, 0, 0, 1), (0, 0, 0, 0, 1)])
+def test_decode_steps_in_which_some_requests_bring_no_token(new):
+    """A request without tokens does not move the rows behind it to other requests' contexts."""
+    pytest.importorskip("vllm")
+    D, Hq, H, bs, n = 128, 8, 2, 16, len(new)
+    impl = B.TurboQuantB200EightBitImpl(Hq, D, 1 / math.sqrt(D), H)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    cache = torch.zeros(B.TurboQuantB200EightBitBackend.get_kv_cache_shape(4 * n, bs, H, D), dtype=torch.uint8, device=DEV)
+    tables = torch.randperm(4 * n, generator=g, device=DEV).view(n, 4).to(torch.int32)
+    lens = [33, 20, 64, 7, 50]
+    layer = SimpleNamespace(layer_name="model.layers.0.self_attn.attn")
+    for i in range(n):
+        k, v = (torch.randn(lens[i], H, D, generator=g, device=DEV).half() for _ in range(2))
+        p = torch.arange(lens[i], device=DEV)
+        impl.do_kv_cache_update(layer, k, v, cache, tables[i].long()[p // bs] * bs + p % bs)
+    T = sum(new)
+    q = torch.randn(T, Hq * D, generator=g, device=DEV).half()
+    step = lambda rows, which, starts: SimpleNamespace(
+        num_actual_tokens=rows, max_query_len=1, query_start_loc=torch.tensor(starts, dtype=torch.int32, device=DEV), block_table=tables[which],
+        seq_lens=torch.tensor([lens[i] for i in which], dtype=torch.int32, device=DEV), max_seq_len=64)
+    starts = [0] + list(torch.tensor(new).cumsum(0))
+    out = impl.forward(layer, q, None, None, cache, step(T, list(range(n)), starts), output=torch.full_like(q, 5.0))
+    there = [i for i in range(n) if new[i]]
+    want = impl.forward(layer, q, None, None, cache, step(T, there, list(range(T + 1))), output=torch.full_like(q, 5.0))
+    assert torch.equal(out, want) and _native.read_status(DEV) == 0

@@ -232,8 +232,10 @@ def _build_classes():
             if attn_metadata is None:
                 return output.fill_(0)
             n = attn_metadata.num_actual_tokens
+            # also where no request has more than one token: one that has none shifts the rows behind it
+            starts = getattr(attn_metadata, "query_start_loc", None)
             most = int(attn_metadata.max_query_len)
-            more = {} if most == 1 else dict(query_start_loc=attn_metadata.query_start_loc, max_query_len=most)
+            more = {} if most == 1 and starts is None else dict(query_start_loc=starts, max_query_len=most)
             res = paged_attention_8bit(query[:n].view(n, self.num_heads, self.head_size), kv_cache, attn_metadata.block_table,
                                        attn_metadata.seq_lens, self._block_size(kv_cache), sm_scale=self.scale,
                                        max_seq_len=int(getattr(attn_metadata, "max_seq_len", 0) or 0), **more)

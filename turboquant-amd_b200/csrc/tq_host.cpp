@@ -464,6 +464,10 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (table.scalar_type() != at::kFloat || table.dim() != 2 || !table.is_contiguous() || table.size(0) < 1 || table.size(1) < 2 ||
         table.size(1) % 2 || table.size(1) > dim || dim > 1 << 20)
         return declined();
+    if (v[0]) {     // interleaved pairs are moved at once: others are copied
+        for (const at::Tensor* x : {&q, &k})
+            if ((address(*x) / x->element_size() | static_cast<uint64_t>(x->stride(0) | x->stride(1) | dim)) % 2) return declined();
+    }
     const at::Device dev = q.device();
     const c10::cuda::CUDAGuard guard(dev);
     at::Tensor q_out = empty(q.sizes(), q.scalar_type(), dev), k_out;

@@ -371,6 +371,17 @@ def _rotary_impl(q, k, q_out, k_out, positions, cos_sin, interleaved: bool, inve
         raise ValueError("rotary_dim must be even and at most head_dim")
     if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.numel() != T or not positions.is_contiguous():
         raise ValueError("positions must be contiguous int32 or int64 with one entry per token")
+    if interleaved and not all(t is None or _pairs_on_their_size(t) for t in (q, k, q_out, k_out)):
+        # The kernel moves a pair at once: the turn is made in copies that are a value wider where a head is odd.
+        copies = [None if t is None else t.new_empty(T, t.shape[1], D + D % 2) for t in (q, k)]
+        for copy, t in zip(copies, (q, k)):
+            if t is not None:
+                copy[..., :D].copy_(t)
+        _rotary_impl(*copies, *copies, positions, cos_sin, interleaved, inverse)
+        for copy, t in zip(copies, (q_out, k_out)):
+            if t is not None:
+                t.copy_(copy[..., :D])
+        return
     zero = (0, 0)
     st = (ctypes.c_int64 * 8)(*q.stride()[:2], *(k.stride()[:2] if k is not None else zero), *q_out.stride()[:2],
                               *(k_out.stride()[:2] if k is not None else zero))
@@ -379,6 +390,11 @@ def _rotary_impl(q, k, q_out, k_out, positions, cos_sin, interleaved: bool, inve
                              int(positions.dtype == torch.int64), _ptr(cos_sin), cos_sin.shape[0], T, q.shape[1],
                              0 if k is None else k.shape[1], D, R, int(interleaved), int(inverse), _ptr(status_word(dev)), _stream(dev))
     _check(rc, "tq_rotary")
+
+
+def _pairs_on_their_size(t: torch.Tensor) -> bool:
+    item = t.element_size()
+    return t.shape[2] % 2 == 0 and (t.data_ptr() | (t.stride(0) | t.stride(1)) * item) % (2 * item) == 0
 
 
 def _quantize8_impl(key, value, cache, slot_mapping, block_size: int) -> None:

@@ -215,3 +215,25 @@ def test_eight_bit_backend():
     assert B.TurboQuantB200Backend.get_impl_cls() is B.TurboQuantB200Impl
     with pytest.raises(NotImplementedError):
         B.TurboQuantB200EightBitImpl(8, 128, 1.0, 2, sliding_window=64)
+
+
+# ---- rows that are not where the kernel can read them -----------------------------------------------------
+def test_rows_are_copied_once_where_they_have_to_be():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Copies(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(func.__name__)
+            return func(*args, **(kwargs or {}))
+
+    flat = torch.arange(5 * 3 * 128 + 8, dtype=torch.float16)
+    for t, copied in ((flat[:-8].view(5, 3, 128), 0), (flat[1:-7].view(5, 3, 128), 1), (flat[:5 * 387].as_strided((5, 3, 128), (385, 128, 1)), 1),
+                      (flat[:-8].view(5, 3, 128)[:, :2, :64], 0)):
+        with Copies() as seen:
+            got = _native._with_aligned_rows(t)
+        assert torch.equal(got, t) and len(seen.names) == copied and (copied or got is t)
+        assert got.data_ptr() % 16 == 0 and all(s * 2 % 16 == 0 for s in got.stride()[:2]) and got.stride(2) == 1

@@ -411,7 +411,7 @@ def _quantize8_impl(key, value, cache, slot_mapping, block_size: int) -> None:
         raise ValueError("cache and key differ in their number of heads")
     if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < T or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be contiguous int64 with at least one entry per token")
-    key, value = (t if _aligned_rows(t) else t.contiguous().clone() for t in (key, value))      # rows are read 16 bytes at a time
+    key, value = (_with_aligned_rows(t) for t in (key, value))
     with torch.cuda.device(dev):
         rc = lib().tq_quantize8_paged(
             _ptr(key), _ptr(value), _DTYPES[key.dtype], key.stride(0), key.stride(1), value.stride(0), value.stride(1), _ptr(cache),
@@ -421,6 +421,11 @@ def _quantize8_impl(key, value, cache, slot_mapping, block_size: int) -> None:
 
 def _aligned_rows(t: torch.Tensor) -> bool:
     return (t.data_ptr() | (t.stride(0) | t.stride(1)) * t.element_size()) % 16 == 0
+
+
+def _with_aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """t, or one copy of it whose rows can be read 16 bytes at a time."""
+    return t if _aligned_rows(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_cache8(cache: torch.Tensor, block_size: int, head_dim: int) -> None:

@@ -29,7 +29,8 @@
 // fp16 weights use their range whatever the scales are (page_weights in tq_attend8.cu has the same two references m and u).
 // A NaN in V counts as zero in the product; its dim and token are noted, and rows that see the token become NaN in that dim at the end.
 //
-// All waits are bounded; one that gives up sets TQ_STATUS_TIMEOUT, every role leaves its loop and the tensor memory is freed.
+// All waits are bounded; one that gives up sets TQ_STATUS_TIMEOUT, every role leaves its loop, copies and products that are under way are waited
+// for, and the tensor memory is freed.
 #pragma once
 
 #include <type_traits>
@@ -71,7 +72,7 @@ struct PromptSmem {
 };
 
 enum PromptBar { kbKFull = 0, kbKEmpty = 2, kbVFull = 4, kbVEmpty = 6, kbSFull = 8, kbPFull = 10, kbPvDone = 12, kbRawKFull = 14, kbRawKEmpty = 15, kbRawVFull = 16, kbRawVEmpty = 17,
-                 kbPlanFull = 18, kbPlanEmpty = 18 + kPlans, kbBars = 18 + 2 * kPlans };
+                 kbPlanFull = 18, kbPlanEmpty = 18 + kPlans, kbDrained = 18 + 2 * kPlans, kbBars };
 static_assert(kbBars * 8 <= 288, "barriers");
 
 __device__ __forceinline__ void prompt_arrive(uint64_t* bar) {
@@ -163,6 +164,14 @@ __device__ __forceinline__ void convert16(uint4 codes, uint32_t at, uint32_t ste
     sts16(at + step, h[4], h[5], h[6], h[7]);
 }
 
+// A whole warp's wait, with one answer for the warp: what follows it is for whole warps.  A role leaves at its own first wait that gives up;
+// those that wait for it give up after it.
+__device__ __forceinline__ bool waited(uint64_t* bar, uint32_t parity, volatile int* flags) {
+    const bool ok = mbar_wait_bounded(bar, parity);
+    if (!ok) flags[0] = 1;
+    return __all_sync(0xffffffffu, ok);
+}
+
 // Lane i < 8 looks at page i of a tile, and has its keys copied, lane 8 + i its values.
 template <int D>
 __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int seq, uint8_t* smem, uint64_t* bars, volatile int* flags) {
@@ -177,7 +186,7 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         const int page = token0 / kPageTokens + mine;
         return page < pages ? __ldg(table + page / p.pages_per_block) : 0;
     };
-    int block = ask_block(job.token_a), step = 0;
+    int block = ask_block(job.token_a), step = 0, keys = 0, values = 0;     // copies of tiles that were issued
     for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
         const int page = token0 / kPageTokens + mine, count = min(pages - token0 / kPageTokens, kTilePages);
         const bool here = mine < count;
@@ -190,15 +199,13 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         const float2 scales = here ? __ldg(reinterpret_cast<const float2*>(at + cache8_scale_off(D))) : make_float2(0.f, 0.f);
         // Pages that are not there keep the codes of another tile: their columns are masked, and finite values times zero are zero.
         const uint32_t turn = (step & 1) ^ 1;
-        if (!mbar_wait_bounded(bars + kbRawKEmpty, turn)) flags[0] = 1;
-        if (flags[0]) break;
+        if (!waited(bars + kbRawKEmpty, turn, flags)) break;
         if (lane == 0) mbar_expect_tx(bars + kbRawKFull, count * kPart);
         __syncwarp();
         if (here && lane < 8) bulk_g2s(smem + Smem::kRawK + mine * kPart, at, kPart, bars + kbRawKFull);
+        ++keys;
         const int slot = step % kPlans;
-        if (!mbar_wait_bounded(bars + kbPlanEmpty + slot, (step / kPlans & 1) ^ 1)) flags[0] = 1;
-        if (!mbar_wait_bounded(bars + kbRawVEmpty, turn)) flags[0] = 1;
-        if (flags[0]) break;
+        if (!waited(bars + kbPlanEmpty + slot, (step / kPlans & 1) ^ 1, flags) || !waited(bars + kbRawVEmpty, turn, flags)) break;
         StepPlan& plan = plans[slot];
         if (lane < kTilePages) {
             plan.k_scale[mine] = scales.x;
@@ -215,7 +222,11 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         }
         __syncwarp();
         if (here && lane >= 8 && lane < 16) bulk_g2s(smem + Smem::kRawV + mine * kPart, at + kPart, kPart, bars + kbRawVFull);
+        ++values;
     }
+    // Nothing is on its way to shared memory when the CTA leaves it, also where the converters have given up.
+    if (keys && !mbar_wait_bounded(bars + kbRawKFull, (keys - 1) & 1)) flags[0] = 1;
+    if (values && !mbar_wait_bounded(bars + kbRawVFull, (values - 1) & 1)) flags[0] = 1;
     if (bad && p.status) atomicOr(p.status, TQ_STATUS_BAD_BLOCK);
 }
 
@@ -237,9 +248,7 @@ __device__ void prompt_convert(const PromptJob& job, uint8_t* smem, uint64_t* ba
     int step = 0;
     for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
         const int s = step & 1;
-        if (!mbar_wait_bounded(bars + kRawFull, step & 1)) flags[0] = 1;
-        if (!mbar_wait_bounded(bars + kEmpty + s, (step >> 1 & 1) ^ 1)) flags[0] = 1;
-        if (flags[0]) return;
+        if (!waited(bars + kRawFull, step & 1, flags) || !waited(bars + kEmpty + s, (step >> 1 & 1) ^ 1, flags)) return;
 #pragma unroll 1
         for (int i = 0; i < kPages; ++i) {
             const int token = (first + i) * kPageTokens + tok;
@@ -295,11 +304,7 @@ __device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* b
     const uint32_t base = smem_u32(smem);
     const int steps = __shfl_sync(0xffffffffu, (job.token_b - job.token_a + kTile - 1) / kTile, 0);
     const bool both = __shfl_sync(0xffffffffu, job.tiles, 0) == 2;
-    auto wait = [&](int bar, uint32_t parity) {
-        if (!mbar_wait_bounded(bars + bar, parity)) flags[0] = 1;
-        __syncwarp();
-        return flags[0] == 0;
-    };
+    auto wait = [&](int bar, uint32_t parity) { return waited(bars + bar, parity, flags); };
     const uint64_t queries = prompt_desc(base + Smem::kQ, 2048, 128), keys = prompt_desc(base + Smem::kK, 2048, 128),
                    values = prompt_desc(base + Smem::kV, D * 16, 128);
     auto scores = [&](int q, int s) {
@@ -314,51 +319,58 @@ __device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* b
             prompt_mma_ts(2 * kTile + q * kTile, q * kTile + i / 4 * 64 + i % 4 * 8, values + (s * Smem::kOperand + i * 2 * (D * 16)) / 16, kOut, i ? 1u : accumulate);
         prompt_commit(bars + kbPvDone + q);
     };
-    if (!wait(kbKFull, 0)) return;
-    prompt_fence_after();
-    if (elect_one()) {
-        scores(0, 0);
-        if (both) scores(1, 0);
-        prompt_commit(bars + kbKEmpty);
-    }
-    __syncwarp();
-    for (int step = 0; step < steps; ++step) {
-        const int s = step & 1, n = s ^ 1;
-        const bool more = step + 1 < steps;
-        if (!wait(kbVFull + s, step >> 1 & 1)) return;
-        if (!wait(kbPFull, step & 1)) return;
+    auto walk = [&]() {
+        if (!wait(kbKFull, 0)) return;
         prompt_fence_after();
         if (elect_one()) {
-            products(0, s, step ? 1u : 0u);
-            if (!both) {
-                prompt_commit(bars + kbVEmpty + s);
-                prompt_commit(bars + kbPlanEmpty + step % kPlans);
-            }
+            scores(0, 0);
+            if (both) scores(1, 0);
+            prompt_commit(bars + kbKEmpty);
         }
         __syncwarp();
-        if (more) {
-            if (!wait(kbKFull + n, (step + 1) >> 1 & 1)) return;
+        for (int step = 0; step < steps; ++step) {
+            const int s = step & 1, n = s ^ 1;
+            const bool more = step + 1 < steps;
+            if (!wait(kbVFull + s, step >> 1 & 1)) return;
+            if (!wait(kbPFull, step & 1)) return;
             prompt_fence_after();
             if (elect_one()) {
-                scores(0, n);
-                if (!both) prompt_commit(bars + kbKEmpty + n);
+                products(0, s, step ? 1u : 0u);
+                if (!both) {
+                    prompt_commit(bars + kbVEmpty + s);
+                    prompt_commit(bars + kbPlanEmpty + step % kPlans);
+                }
+            }
+            __syncwarp();
+            if (more) {
+                if (!wait(kbKFull + n, (step + 1) >> 1 & 1)) return;
+                prompt_fence_after();
+                if (elect_one()) {
+                    scores(0, n);
+                    if (!both) prompt_commit(bars + kbKEmpty + n);
+                }
+                __syncwarp();
+            }
+            if (!both) continue;
+            if (!wait(kbPFull + 1, step & 1)) return;
+            prompt_fence_after();
+            if (elect_one()) {
+                products(1, s, step ? 1u : 0u);
+                prompt_commit(bars + kbVEmpty + s);
+                prompt_commit(bars + kbPlanEmpty + step % kPlans);              // the softmax warps are done with it, too
+                if (more) {
+                    scores(1, n);
+                    prompt_commit(bars + kbKEmpty + n);
+                }
             }
             __syncwarp();
         }
-        if (!both) continue;
-        if (!wait(kbPFull + 1, step & 1)) return;
-        prompt_fence_after();
-        if (elect_one()) {
-            products(1, s, step ? 1u : 0u);
-            prompt_commit(bars + kbVEmpty + s);
-            prompt_commit(bars + kbPlanEmpty + step % kPlans);              // the softmax warps are done with it, too
-            if (more) {
-                scores(1, n);
-                prompt_commit(bars + kbKEmpty + n);
-            }
-        }
-        __syncwarp();
-    }
+    };
+    walk();
+    // No product is under way when tensor memory is freed, also where the softmax warps have given up.
+    if (elect_one()) prompt_commit(bars + kbDrained);
+    __syncwarp();
+    wait(kbDrained, 0);
 }
 
 constexpr float kTiny = 1e-38f;             // factors of scores are never zero: times -inf that would be NaN
@@ -402,9 +414,8 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
     bool ok = true;
     int step = 0;
     for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
-        if (!mbar_wait_bounded(bars + kbPlanFull + step % kPlans, step / kPlans & 1)) flags[0] = 1;
-        if (!mbar_wait_bounded(bars + kbSFull + q, step & 1)) flags[0] = 1;
-        __syncwarp();                                                        // what follows is for whole warps
+        bool lost = !waited(bars + kbPlanFull + step % kPlans, step / kPlans & 1, flags);
+        lost |= !waited(bars + kbSFull + q, step & 1, flags);
         prompt_fence_after();
         const StepPlan& plan = plans[step % kPlans];
         const int visible = limit - token0 - 64 * half;
@@ -464,7 +475,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
             if (again) break;
             // Both warps of the rows decide alike, also about giving up.
             const int mine = __any_sync(0xffffffffu, most > m + kLazy || most_v > u + kLazy) ? 1 : 0;
-            if (lane == 0) over[(step & 1) * 16 + half] = mine | (flags[0] ? 2 : 0);
+            if (lane == 0) over[(step & 1) * 16 + half] = mine | (lost ? 2 : 0);
             __syncwarp();
             asm volatile("bar.sync %0, 64;" ::"r"(1 + together) : "memory");
             const int both = over[(step & 1) * 16] | over[(step & 1) * 16 + 1];
@@ -479,8 +490,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
             u = u1;
             if (step) {
                 // O is whole when the product of the step before is done
-                if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
-                __syncwarp();
+                waited(bars + kbPvDone + q, (step - 1) & 1, flags);
                 prompt_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < D / 32; ++h) {
@@ -517,11 +527,11 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
         if (lane == 0) prompt_arrive(bars + kbPFull + q);
     }
     if (ok && step) {
-        if (!mbar_wait_bounded(bars + kbPvDone + q, (step - 1) & 1)) flags[0] = 1;
+        ok = waited(bars + kbPvDone + q, (step - 1) & 1, flags);
         prompt_fence_after();
     }
     __syncwarp();
-    ok = ok && flags[0] == 0;
+    ok = ok && __all_sync(0xffffffffu, flags[0] == 0);
     asm volatile("bar.sync %0, 64;" ::"r"(1 + together) : "memory");
     l += exchange(row_slot, half, 1 + together, l);
     // The row's values: in units of the weights' reference, divided by their sum where this CTA saw all of them.
@@ -685,6 +695,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend8_prompt_kernel(const
             mbar_init(bars + kbPFull + i, 8);
             mbar_init(bars + kbPvDone + i, 1);
         }
+        mbar_init(bars + kbDrained, 1);
         mbar_init(bars + kbRawKFull, 1);
         mbar_init(bars + kbRawKEmpty, 2);
         mbar_init(bars + kbRawVFull, 1);

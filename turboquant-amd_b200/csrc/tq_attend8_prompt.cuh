@@ -47,7 +47,7 @@ constexpr int kPlans = 8;
 constexpr int kRankedSeqs = 128;                // sequences that a CTA sorts by length
 
 // The scales of a tile's pages: of K as it is, of V as the power of two.
-struct StepPlan {
+struct alignas(16) StepPlan {
     float k_scale[kTilePages], v_exp[kTilePages];
     int token0, last, pad[2];
 };
@@ -68,7 +68,7 @@ struct PromptSmem {
     static constexpr int kRawK = kV + 2 * kOperand;                      // codes of a tile's keys, values
     static constexpr int kRawV = kRawK + kTile * D;
     static constexpr int kBytes = kRawV + kTile * D;
-    static_assert(kRows + 8 * 32 * 4 <= kQ && kBytes <= 227 * 1024, "shared memory map");
+    static_assert(kPlan % 16 == 0 && kRows + 8 * 32 * 4 <= kQ && kBytes <= 227 * 1024, "shared memory map");
 };
 
 enum PromptBar { kbKFull = 0, kbKEmpty = 2, kbVFull = 4, kbVEmpty = 6, kbSFull = 8, kbPFull = 10, kbPvDone = 12, kbRawKFull = 14, kbRawKEmpty = 15, kbRawVFull = 16, kbRawVEmpty = 17,
@@ -456,21 +456,27 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
                         z = ex2(z);
                         w[8 * g + i] = pack_half2(y, z);
                         if (!BF16) {
-                            // as page_weights does; an output in bf16 does not show the difference
+                            // as they are rounded for the product (counted()); an output in bf16 does not show the difference
                             const float2 v = unpack_half2(w[8 * g + i]);
-                            y = counted(y, v.x);
-                            z = counted(z, v.y);
+                            y = decltype(cut)::value ? counted(y, v.x) : v.x;
+                            z = decltype(cut)::value ? counted(z, v.y) : v.y;
                         }
                         sums = add2(sums, pair(y, z));
                     }
                     float sum0, sum1;
                     unpair(sums, sum0, sum1);
-                    const float up = u - ev - m;                             // the sum in units of m again; page_weights
+                    const float up = u - ev - m;
                     far |= up > kFarApart;
-                    sum = fmaf(sum0 + sum1, up > kFarApart ? 0.f : ex2(up - kHeadroom), sum);
+                    sum = fmaf(sum0 + sum1, up > kFarApart ? 0.f : ex2(up - kHeadroom), sum);   // in units of m again
                 }
             };
-            if (masked) pass(std::true_type{});
+            // the rarer code also looks at what each weight counts for
+            bool apart = false;
+            if constexpr (!BF16) {
+                const float4 ev = *reinterpret_cast<const float4*>(plan.v_exp + 4 * half);
+                apart = __any_sync(0xffffffffu, u - m - fminf(fminf(ev.x, ev.y), fminf(ev.z, ev.w)) > kLossless);
+            }
+            if (masked || apart) pass(std::true_type{});
             else pass(std::false_type{});
             if (again) break;
             // Both warps of the rows decide alike, also about giving up.

@@ -79,11 +79,14 @@ def gather(codes, scales, table, length, block_size, h, kv):
 def attention(q, codes, scales, tables, lens, starts, block_size, sm_scale, eps):
     """(out, tolerance) of paged_attention_8bit for q [T, Hq, D] in 64 bits.
 
-    The tolerance of an output is half a step eps / 2 of its type, plus sum_k w_k |v_k| times what the weights are off:
-    2^-11 for their rounding to fp16 (half a step is 2^-12, the largest weight of a page may lie below the reference it
-    is rounded against only where it is normal), and 2 ln 2 times the error of a score in units of log2 (numerator and denominator): D
-    fp32 additions and products, 2^-24 each, of the sum of |q k|; a few roundings of the score itself; for queries in
-    bf16 values below 2^-14 of the row's largest are off by 2^-25 of it.  Weights below 2^-31 of the largest may vanish.
+    The tolerance of an output is half a step eps / 2 of its type, plus what the weights w_k are off.
+    * Their rounding to fp16, at most 2^-11 of a weight (half a step).  Where the denominator sums rounded weights, the output is
+      sum w_k (1 + d_k) v_k / sum w_k (1 + d_k), off by sum w_k d_k (v_k - out) to first order; where it sums them as they are, by
+      sum w_k d_k v_k.  Both are at most 2^-11 (sum w_k |v_k| + |out|).
+    * 2 ln 2 times the error of a score in units of log2 (numerator and denominator), relative to sum_k w_k |v_k|: D fp32 additions and
+      products, 2^-24 each, of the sum of |q k|; a few roundings of the score itself; for queries in bf16 values below 2^-14
+      of the row's largest are off by 2^-25 of it.
+    * Weights below 2^-30 of the largest may vanish.
     """
     T, Hq, D = q.shape
     G = Hq // codes.shape[1]
@@ -106,9 +109,9 @@ def attention(q, codes, scales, tables, lens, starts, block_size, sm_scale, eps)
                     w /= w.sum(1, keepdims=True)
                     out[a + j, h * G:(h + 1) * G] = w @ v[:L]
                     size = np.abs(x) @ np.abs(k[:L]).T + 2.0 ** -1 / D * np.abs(x).max(1, keepdims=True) * np.abs(k[:L]).sum(1)
-                    off = (sm_scale * size * (D + 8) * 2.0 ** -24).max(1) * 2 + 2.0 ** -20 + 2.0 ** -11
+                    off = (abs(sm_scale) * size * (D + 8) * 2.0 ** -24).max(1) * 2 + 2.0 ** -20 + 2.0 ** -11
                     most = np.abs(v[:L]).max(0)
-                    tol[a + j, h * G:(h + 1) * G] = off[:, None] * (w @ np.abs(v[:L])) + L * 2.0 ** -30 * most
+                    tol[a + j, h * G:(h + 1) * G] = off[:, None] * (w @ np.abs(v[:L])) + 2.0 ** -11 * np.abs(out[a + j, h * G:(h + 1) * G]) + L * 2.0 ** -30 * most
     return out, tol + np.abs(out) * eps / 2 + 2.0 ** -24
 
 

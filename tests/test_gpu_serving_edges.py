@@ -158,3 +158,32 @@ def test_offsets_that_are_none_touch_nothing_else():
     paged_attention_8bit(q, cache, tables, torch.tensor([64, 64, 64], **i32), 16, query_start_loc=wild, max_query_len=2, out=around[3:6])
     assert _native.read_status(DEV) == _native.STATUS_TOO_LONG
     assert (around[:3] == 7).all() and (around[5:] == 7).all() and torch.isfinite(around).all()
+
+
+# ---- scales and sizes in the kernel for prompt chunks ------------------------------------------------------
+def test_prompt_chunks_with_negative_and_zero_scales():
+    for dtype in (torch.float16, torch.bfloat16):
+        _check_attention(gen(5), [300, 40], [40, 40], 8, 2, 128, 16, dtype, sm_scale=-0.05)
+        _check_attention(gen(6), [300, 40], [40, 40], 8, 2, 128, 16, dtype, sm_scale=0.0)
+
+
+def test_prompt_chunks_with_scores_of_any_size():
+    _check_attention(gen(1), [300, 40], [40, 40], 8, 2, 128, 16, torch.float16, q_size=30.0, spread=0, sm_scale=0.02)
+    _check_attention(gen(2), [300, 40], [40, 40], 8, 2, 128, 16, torch.bfloat16, spread=40, sm_scale=2.0 ** -45)
+    _check_attention(gen(3), [300, 40], [40, 40], 8, 2, 128, 16, torch.bfloat16, q_size=1e30, sm_scale=1e-32)
+    _check_attention(gen(4), [300, 40], [40, 40], 8, 2, 128, 16, torch.bfloat16, q_size=1e-30, sm_scale=1e28)
+
+
+# ---- repetition --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("queries,lens,width", [([1], [5000], 0), ([1] * 40, [700] * 40, 0), ([1] * 30, [100 * i + 1 for i in range(30)], 9000),
+                                                ([300, 200], [3000, 900], 0), ([1, 1, 300, 2, 1], [900, 70, 1200, 33, 400], 9000)])
+def test_repeated_calls_are_equal_bit_for_bit(queries, lens, width):
+    g = gen(len(queries))
+    cache, tables = _filled(g, lens, 2, 128, 16)
+    tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+    q = torch.randn(sum(queries), 16, 128, generator=g, device=DEV).half()
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(queries)]), **i32)
+    call = lambda: paged_attention_8bit(q, cache, tables, torch.tensor(lens, **i32), 16, query_start_loc=starts, max_query_len=max(queries))
+    first = call()
+    for _ in range(20):
+        assert torch.equal(call(), first)

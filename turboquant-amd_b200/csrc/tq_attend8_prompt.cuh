@@ -49,7 +49,6 @@ constexpr int kRankedSeqs = 128;                // sequences that a CTA sorts by
 // The scales of a tile's pages: of K as it is, of V as the power of two.
 struct alignas(16) StepPlan {
     float k_scale[kTilePages], v_exp[kTilePages];
-    int token0, last, pad[2];
 };
 
 template <int D>
@@ -210,10 +209,6 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         if (lane < kTilePages) {
             plan.k_scale[mine] = scales.x;
             plan.v_exp[mine] = here ? static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127) : 0.f;
-        }
-        if (lane == 0) {
-            plan.token0 = token0;
-            plan.last = token0 + kTile >= job.token_b;
         }
         __syncwarp();
         if (lane == 0) {

@@ -8,6 +8,7 @@ import torch
 from oracle import serving_oracle as S
 from test_gpu_serving_ops import DEV, EPS, _check_attention, _filled, _state, clean_status, gen, i32  # noqa: F401  (an autouse fixture)
 from turboquant.kernels import _native
+from turboquant.kernels.block_plan import plan_step, release_blocks
 from turboquant.kernels.paged_8bit import allocate_cache_8bit, codes_and_scales, paged_attention_8bit
 
 pytestmark = pytest.mark.gpu
@@ -187,3 +188,90 @@ def test_repeated_calls_are_equal_bit_for_bit(queries, lens, width):
     first = call()
     for _ in range(20):
         assert torch.equal(call(), first)
+
+
+# ---- calls that nothing above makes ----------------------------------------------------------------------------
+@pytest.mark.parametrize("Hq,H,n,width", [(33, 1, 5, 0), (71, 1, 5, 0), (128, 1, 3, 9000), (257, 1, 3, 0), (80, 2, 140, 0), (40, 1, 900, 0)])
+def test_single_queries_of_large_groups(Hq, H, n, width):
+    """More than 32 query heads on a KV head: single tokens in the kernel for prompt chunks, without offsets, up to more sequences than are ranked."""
+    lens = [(37 * i) % 200 for i in range(n - 1)] + [700]
+    _check_attention(gen(Hq), lens, [1] * n, Hq, H, 64, 16, torch.bfloat16 if n > 10 else torch.float16, width=width)
+
+
+@pytest.mark.parametrize("n,width", [(1, 0), (1, 20000), (3, 0), (3, 20000), (30, 0)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_query_that_is_no_number_spoils_its_own_row_only(n, width, dtype):
+    g = gen(n)
+    cache, tables = _filled(g, [300, 90], 2, 128, 16)
+    tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+    q = torch.randn(2 * n, 8, 128, generator=g, device=DEV).to(dtype)
+    more = {} if n == 1 else dict(query_start_loc=torch.tensor([0, n, 2 * n], **i32), max_query_len=n)
+    lens = torch.tensor([300, 90], **i32)
+    clean = paged_attention_8bit(q, cache, tables, lens, 16, **more)
+    q[0, 3, 17], q[2 * n - 1, 5, 100] = math.nan, math.inf
+    got = paged_attention_8bit(q, cache, tables, lens, 16, **more)
+    spoilt = torch.zeros(2 * n, 8, dtype=torch.bool, device=DEV)
+    spoilt[0, 3] = spoilt[2 * n - 1, 5] = True
+    assert got[spoilt].isnan().all() and torch.equal(got[~spoilt], clean[~spoilt])
+
+
+@pytest.mark.parametrize("queries,lens,width", [([1] * 9, [900] * 9, 0), ([1] * 20, [100 * i + 1 for i in range(20)], 9000), ([90, 40], [3000, 100], 0),
+                                                ([1, 1, 200, 2], [900, 70, 700, 33], 9000)])
+def test_the_result_may_take_the_queries_place(queries, lens, width):
+    g = gen(len(queries))
+    cache, tables = _filled(g, lens, 2, 64, 16)
+    tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+    q = torch.randn(sum(queries), 12, 64, generator=g, device=DEV).half()
+    call = dict(query_start_loc=torch.tensor(np.concatenate([[0], np.cumsum(queries)]), **i32), max_query_len=max(queries))
+    want = paged_attention_8bit(q, cache, tables, torch.tensor(lens, **i32), 16, **call)
+    assert paged_attention_8bit(q, cache, tables, torch.tensor(lens, **i32), 16, out=q, **call) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("queries,lens,width", [([1] * 30, [100 * i + 1 for i in range(30)], 9000), ([300, 200], [3000, 900], 0), ([1, 1, 300, 2], [900, 70, 1200, 33], 9000)])
+def test_two_calls_at_once(queries, lens, width):
+    """Calls on two streams, each with a workspace of its own: those of one do not show in the other's."""
+    problems = []
+    for seed in (1, 2):
+        g = gen(seed)
+        cache, tables = _filled(g, lens, 2, 128, 16)
+        tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+        q = torch.randn(sum(queries), 16, 128, generator=g, device=DEV).half()
+        starts = torch.tensor(np.concatenate([[0], np.cumsum(queries)]), **i32)
+        args, kw = (q, cache, tables, torch.tensor(lens, **i32), 16), dict(query_start_loc=starts, max_query_len=max(queries))
+        problems.append((args, kw, paged_attention_8bit(*args, **kw)))
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(15):
+        for stream, (args, kw, _), out in zip(streams, problems, outs):
+            with torch.cuda.stream(stream):
+                out.append(paged_attention_8bit(*args, **kw))
+    torch.cuda.synchronize()
+    for (_, _, want), out in zip(problems, outs):
+        assert all(torch.equal(o, want) for o in out)
+
+
+# ---- numbers beyond 32 bits --------------------------------------------------------------------------------
+@pytest.mark.parametrize("most", [100, (1 << 27) + 5, (1 << 31) - 1, (1 << 32) + 1, 1 << 40])
+def test_any_bound_of_the_queries_will_do(most):
+    """max_query_len only has to be large enough."""
+    g = gen(8)
+    cache, tables = _filled(g, [40, 300, 9], 2, 64, 16)
+    q = torch.randn(6, 64, 64, generator=g, device=DEV).half()
+    starts, lens = torch.tensor([0, 1, 4, 6], **i32), torch.tensor([40, 300, 9], **i32)
+    want = paged_attention_8bit(q, cache, tables, lens, 16, query_start_loc=starts, max_query_len=3)
+    c, s = _state(cache, 16, 64)
+    ref, tol = S.attention(q.double().cpu().numpy(), c, s, tables.cpu().numpy(), [40, 300, 9], [0, 1, 4, 6], 16, 0.125, EPS[torch.float16])
+    assert (np.abs(want.double().cpu().numpy() - ref) <= tol).all()
+    for out in (None, torch.full_like(q, 7.0)):
+        got = paged_attention_8bit(q, cache, tables, lens, 16, query_start_loc=starts, max_query_len=most, out=out)
+        assert (np.abs(got.double().cpu().numpy() - ref) <= tol).all() and (out is None or got is out)
+
+
+def test_block_sizes_beyond_32_bits_are_refused():
+    v, t, c = torch.ones(2, **i32), torch.zeros(2, 4, **i32), torch.ones(1, **i32)
+    with pytest.raises(ValueError, match="block_size"):
+        plan_step(v, v, t, v, c, (1 << 32) + 16, 2)
+    with pytest.raises(ValueError, match="block_size"):
+        release_blocks(v.bool(), v, t, v, c, (1 << 32) + 16)

@@ -525,13 +525,14 @@ PyObject* attend8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != 10 || !plain_eager() || !tensors_on_one_device(args, t) || !floats(args + 6, 1, scale) || !ints(args + 7, 3, v)) return declined();
     const at::Tensor &q = *t[0], &cache = *t[1], &tables = *t[2], &lens = *t[3];
     int32_t* status = status_of(q);
-    const long long block_size = v[0], max_queries = v[1], max_len = v[2];
+    const long long block_size = v[0], max_len = v[2];
+    long long max_queries = v[1];
     const int dtype = dtype_code(q);
     if (!status || (dtype != TQ_DTYPE_F16 && dtype != TQ_DTYPE_BF16) || q.dim() != 3 || !q.is_contiguous() || address(q) % 16) return declined();
     const int64_t T = q.size(0), hq = q.size(1), dim = q.size(2);
     if (!is_cache8(cache, block_size, dim)) return declined();
     const int64_t hkv = cache.size(1);
-    if (hkv < 1 || hq < 1 || hq % hkv || cache.size(0) < 1 || hq > INT32_MAX || max_queries < 1 || max_queries > INT32_MAX) return declined();
+    if (hkv < 1 || hq < 1 || hq % hkv || cache.size(0) < 1 || hq > INT32_MAX || T > INT32_MAX || max_queries < 1) return declined();
     int64_t ns = T;
     const int32_t* starts = nullptr;
     auto other = [&](PyObject* obj) -> const at::Tensor* {
@@ -546,6 +547,7 @@ PyObject* attend8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     } else if (max_queries != 1) {
         return declined();
     }
+    max_queries = std::min<long long>(max_queries, std::max<int64_t>(T, 1));      // no sequence has more
     if (ns > INT32_MAX || !is_table(tables, ns) || lens.scalar_type() != at::kInt || !lens.is_contiguous() || lens.numel() < ns) return declined();
     void* out_ptr = nullptr;
     if (args[5] != Py_None) {

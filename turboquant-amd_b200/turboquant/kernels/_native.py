@@ -465,6 +465,7 @@ def _attend8_impl(out, q, cache, block_tables, seq_lens, query_start_loc, sm_sca
         ns = query_start_loc.numel() - 1
     if max_query_len < 1:
         raise ValueError("max_query_len must be positive")
+    max_query_len = min(int(max_query_len), max(T, 1))            # no sequence has more
     if seq_lens.numel() < ns or block_tables.shape[0] < ns:
         raise ValueError("seq_lens and block_tables need an entry for every sequence")
     if T and ns and nb < 1:
@@ -497,8 +498,8 @@ def _check_requests(lens, block_tables, free_blocks, free_count, block_size: int
         raise ValueError("one length and one row of block_tables per request, free_count of one element")
     if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
         raise ValueError("block_tables must have contiguous rows")
-    if block_size < 1:
-        raise ValueError("block_size must be positive")
+    if not 1 <= block_size < 1 << 31:
+        raise ValueError("block_size must be positive and fit 32 bits")
     return n
 
 

@@ -5,7 +5,8 @@
 //   s_k = sm_scale * <q, K_k> * kscale(page of k)      for k < len - n + j + 1
 //   out = sum_k 2^(s_k - m) vscale(page of k) V_k / sum_k 2^(s_k - m)      (s in units of log2)
 //
-// Bound: HBM, the 2 D + 2 bytes of a cached token and head, at about D / 16 products and 70 other instructions a page and warp.
+// Bound: HBM, the 2 D + 2 bytes of a cached token and head.  8 query rows take D / 8 products (m16n8k16) a page of 16 tokens; with D = 128 the persistent
+// kernel issues 348 warp instructions a page in all, at half of the issue slots.
 #include "tq_cache8.cuh"
 
 namespace tq {
@@ -656,15 +657,17 @@ struct Attend8Plan {
     int small_rows;                     // kPrompt: sequences of at most so many rows are left to the persistent kernel
 };
 
-// The persistent kernel needs a page or two per warp of the GPU at least.  (8 KV heads, 64 sequences of 512 tokens: 22.3 us, 16.0 in
-// clusters; 64 of 1024: 36.4, 31.9; one of 65536: 37.6, 54.7.)
+// The persistent kernel takes launches of so many pages, 14 for each warp of the GPU.  It gains by sharing out few long items, or a few more than fill
+// the GPU once; where clusters fill it evenly they are ahead up to about 100000 pages, and one line by pages cannot have both.  In us, clusters / persistent,
+// 64 / 8 heads, fp16, n sequences of so many tokens: above the line 64 x 1024 32.1 / 37.3, 64 x 2048 57.0 / 58.8, 64 x 4096 106.0 / 101.7, 1 x 65536
+// 52.6 / 38.2, 16 x 4096 31.4 / 36.0, 20 x 4096 80.7 / 41.5; below it 64 x 512 19.2 / 25.5, 4 x 4096 13.7 / 18.4, 20 x 2048 43.5 / 27.8.
 constexpr int64_t kStreamPages = 32768;
 
 // Which kernel, and how it is cut.
 Attend8Plan attend8_plan(int64_t num_rows, int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
     Attend8Plan a = {};
     const int64_t rows = static_cast<int64_t>(group) * max_queries;
-    // (64 x 8192 tokens, 64 / 8 heads: 32 rows are 456 us in tiles of 16 rows, 64 rows 600 in one tile of 256.)
+    // (64 x 8192 tokens, 64 / 8 heads: 32 rows are 427 us in tiles of 16 rows, 64 rows 667 in one tile of 256, both fp16.)
     if (rows > 32) {
         a.kind = Attend8Kind::kPrompt;
         a.tiles = (rows + 2 * kTile - 1) / (2 * kTile) * seqs;
@@ -672,7 +675,7 @@ Attend8Plan attend8_plan(int64_t num_rows, int64_t seqs, int kv_heads, int group
         if (full + seqs < a.tiles) a.tiles = full + seqs;
         int64_t items = a.tiles;
         // Decodes next to a chunk: a tile of 256 rows with 4 or 8 in use costs what a full one does.  (32 / 8 heads, 64 decodes over 8192 tokens and a
-        // chunk of 2048: 599 us, 1222 by one kernel; 200 over 1024 and two of 1024: 205, 639; 8 over 4096 and four of 512: 275, 288.)
+        // chunk of 2048: 605 us, 1222 by one kernel; 200 over 1024 and two of 1024: 206, 639; 8 over 4096 and four of 512: 271, 288.)
         if (group <= 16 && num_rows < seqs * max_queries && seqs * kv_heads * max_pages >= kStreamPages) {
             a.small_rows = 16;
             a.nt = group <= 8 ? 1 : 2;

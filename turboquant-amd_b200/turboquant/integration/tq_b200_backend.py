@@ -11,15 +11,16 @@ prefill runs ordinary attention on the raw K/V of the step.  Differences:
   * the cache tensor is uint8 [num_blocks, num_kv_heads, block_size/16 * page_bytes]
     (TurboQuant packed pages), not FP4 nibbles plus side buffers of scales.
 
-A second backend, TurboQuantB200EightBitBackend, keeps a layer's keys and values in 8 bits (paged_8bit): for the protected boundary
-layers, which the packed cache leaves out, and for steps that continue cached context with several tokens, which it serves like
-any other (the reference's extend branch, tq_fp4_backend.py:555-601).
+A second backend, TurboQuantB200EightBitBackend, keeps keys and values in 8 bits (paged_8bit) and serves decodes, fresh prompts and
+chunks that continue cached context alike (the reference's extend branch, tq_fp4_backend.py:555-601).  `register(eight_bit=True)`
+makes it the engine's backend for every layer; nothing here gives the layers of one model different backends.
 
 The classes are built on first use so that importing this module does not import vLLM.
 Status: written against vLLM 0.22's v1 interface.  `do_kv_cache_update` and `forward` are exercised
 on a GPU with hand-built layer and metadata objects (decode, fresh prefill and steps that mix both);
-they have not been run inside a vLLM engine.  A step may mix decode rows (one new token over cached
-context) with fresh prefills; a prefill chunk that continues cached context (an "extend") raises.
+they have not been run inside a vLLM engine.  In the packed backend a step may mix decode rows (one new
+token over cached context) with fresh prefills; a prefill chunk that continues cached context (an
+"extend") and protected boundary layers raise there.
 """
 from __future__ import annotations
 

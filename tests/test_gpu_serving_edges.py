@@ -15,13 +15,16 @@ pytestmark = pytest.mark.gpu
 
 
 # ---- denominators --------------------------------------------------------------------------------------
-def _one_token_and_many(far, key, N, dtype, n, H, seqs, width, value=1.0):
-    """Token 0 with score 0 and value scale `value`; N tokens with score `key` in pages whose value scale is 2^far smaller.  All sequences and heads are alike."""
+def _one_token_and_many(far, key, N, dtype, n, H, seqs, width, value=1.0, lone=False):
+    """Token 0 with score 0 and value scale `value`; N tokens with score `key` in pages whose value scale is 2^far smaller.  All sequences and heads are alike.
+    lone: token 0 has values in four dims only."""
     D, bs = 64, 16
     cache = allocate_cache_8bit(9, bs, H, DEV, D)
     codes, scales = codes_and_scales(cache, bs, D)
     g = gen(N)
     codes[:, :, :, 1] = (torch.randn(9, 1, 1, 16, D, generator=g, device=DEV) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    if lone:
+        codes.view(torch.uint8)[0, :, :, 1, :, 4:] = 0
     codes[1:, :, :, 0, :, 0] = torch.tensor(float(key), device=DEV).to(torch.float8_e4m3fn)
     codes[0, :, :, 0, 1:, 0] = torch.tensor(-448.0, device=DEV).to(torch.float8_e4m3fn)      # the other tokens of its page: weight e^-448
     scales[..., 0], scales[0, ..., 1], scales[1:, ..., 1] = 1.0, value, value * 2.0 ** -far
@@ -58,6 +61,39 @@ def test_denominators_keep_small_weights_of_small_values(far, key, N, dtype, n, 
 def test_denominators_of_value_scales_as_far_apart_as_they_get(far, value, key, n, H, seqs, width):
     """Pages of zeros have the least scale, 2^-100: their weights count whatever the scale of the others is."""
     _one_token_and_many(far, key, 1024, torch.bfloat16, n, H, seqs, width, value)
+
+
+@_KERNELS
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("far,key,N,value", [(16, -11, 2048, 64.0), (16, -11, 8192, 64.0), (14, -12, 8192, 64.0), (12, -14, 65536, 16.0), (8, -16, 131072, 4.0),
+                                             (3, -20, 131072, 1.0), (2, -20, 131072, 1.0), (10, -3, 704, 16.0), (20, -9, 4096, 64.0), (22, -6, 1024, 128.0)])
+def test_small_values_beside_zeros_of_a_page_of_large_ones(far, key, N, value, dtype, n, H, seqs, width):
+    """In dims in which the large page holds zeros the output is made of the small values alone, at weights that are tiny next to its."""
+    _one_token_and_many(far, key, N, dtype, n, H, seqs, width, value, lone=True)
+
+
+@pytest.mark.parametrize("n,width", [(1, 0), (1, 40000), (4, 40000), (40, 0)])
+@pytest.mark.parametrize("steps", [(0, -14, 3, -20, 0, -6, 5, -9), (5, 0, -6, -12, -17, 2, -8, -15), (-16, 0, -15, 1, -14, 2, -13, 3)])
+def test_value_scales_that_rise_and_fall(steps, n, width):
+    """Pages whose value scales go up and down by many powers of two, with values in dims of their own beside common ones: every page's dims are right."""
+    g = gen(len(steps) + n)
+    D, bs, H, L = 64, 16, 2, 1536
+    cache, tables = _filled(g, [L], H, D, bs, spread=0)
+    codes, scales = codes_and_scales(cache, bs, D)
+    raw = codes.view(torch.uint8)
+    for page in range(L // bs):
+        k, b = page % len(steps), int(tables[0, page])
+        scales[b, :, 0, 1] = 2.0 ** (steps[k] - 4)
+        raw[b, :, 0, 1, :, 8:] &= 0x80
+        raw[b, :, 0, 1, :, 8 + 7 * k:15 + 7 * k] |= torch.randint(0x30, 0x78, (H, 16, 7), generator=g, device=DEV, dtype=torch.uint8)
+    tables = torch.nn.functional.pad(tables, (0, width), value=-9)
+    q = (torch.randn(n, 4 * H, D, generator=g, device=DEV) * 2).half()
+    more = {} if n == 1 else dict(query_start_loc=torch.tensor([0, n], **i32), max_query_len=n)
+    got = paged_attention_8bit(q, cache, tables, torch.tensor([L], **i32), bs, **more)
+    c, s = _state(cache, bs, D)
+    want, tol = S.attention(q.double().cpu().numpy(), c, s, tables.cpu().numpy(), [L], [0, n], bs, D ** -0.5, EPS[torch.float16])
+    off = np.abs(got.double().cpu().numpy() - want) / tol
+    assert off.max() <= 1, off.max((0, 1))
 
 
 # ---- NaN -----------------------------------------------------------------------------------------------

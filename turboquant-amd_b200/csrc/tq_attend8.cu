@@ -29,8 +29,7 @@ struct Attend8Params {
 
 constexpr float kNothing = -3e38f;      // reference of a row that has seen no token: below every score, and finite, so that differences are numbers
 constexpr float kLazy = 8.f;            // a score may pass the reference by so much before it is raised
-constexpr float kFarApart = 64.f;       // value scales so many powers of two apart: page_weights
-constexpr float kHeadroom = 6.f;        // weights are multiplied by 2^6: at most 2^14 in fp16, full precision down to 2^-20 of the largest
+constexpr float kHeadroom = 7.f;        // weights are multiplied by 2^7: at most 2^15 in fp16, full precision down to 2^-21 of the largest
 
 // What one warp holds while it walks over pages of a sequence, for 8 * NT query rows against one KV head.
 //
@@ -234,17 +233,13 @@ __device__ __forceinline__ bool has_nan(const Page<D>& x, int from, int lane) {
     return __any_sync(0xffffffffu, found != 0);
 }
 
-// What a weight in units of the values' reference counts for in the denominator.  That is the weight as it was rounded for the product, so that a
-// rounding common to both cancels and a token that takes nearly all is exact.  But fp16 has no full precision below 2^-14 and nothing below 2^-25: where
-// the page's values are 2^up below the reference, that is every weight below 2^(up - 31) of the largest, and there may be many
-// of them.  Such a weight counts as it is, where `up` is above kLossless: what is lost below that, 2^-30 of the largest value for each token, is
-// lost in the product as well.  (Looked at for every page: 64 x 2 tokens over 8192, 64 / 8 heads, 240 us; 227 behind a vote that pages of like scales do not pass.)
-constexpr float kLossless = 1.01f;         // value scales a factor of two apart, with what rounding makes of the difference
-__device__ __forceinline__ float counted(float weight, float rounded) { return weight < 6.103515625e-5f ? weight : rounded; }
+// A page's value scale may lie so many powers of two below the reference: fp16 then holds weights down to 2^-30 of the largest, and what is lost is
+// 2^-30 of the values for each token.  (Two, one of which the reference's rounding up may take, and what rounding makes of the difference.)
+constexpr float kLossless = 2.01f;
 
-// One page.  The softmax keeps two references per column: m for the denominators and u, which includes the value scale 2^ev of the page, for the
-// products, whose fp16 weights then use their range whatever the pages' scales are.  Both are raised only where a score passes
-// them by 2^8: most pages need one vote and no shuffles.
+// One page.  The softmax keeps two references per column: m for the denominators and u, a whole number, which includes the value scale 2^ev of the page, for
+// the products, whose fp16 weights then use their range whatever the pages' scales are.  Both are raised only where a score passes
+// them by 2^8: most pages need two votes and no shuffles.
 template <int D, int NT>
 __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], float2 scales, int page, uint32_t (&weights)[NT][2]) {
     const int g = (threadIdx.x & 31) >> 2;
@@ -276,9 +271,9 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
                 float most = fmaxf(s[n][j], s[n][j + 2]) * c[n][j];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float m = fmaxf(w.m[n][j], most), u = fmaxf(w.u[n][j], most + ev);
+                const float m = fmaxf(w.m[n][j], most), u = fmaxf(w.u[n][j], ceilf(most + ev));
                 w.l[n][j] *= ex2(w.m[n][j] - m);
-                const float down = ex2(w.u[n][j] - u);
+                const float down = exp2_int(static_cast<int>(fmaxf(w.u[n][j] - u, -127.f)));        // exact; 2^-127 is zero
 #pragma unroll
                 for (int i = 0; i < Rows<D, NT>::kSteps; ++i) {
                     w.o[i][n][j] *= down;
@@ -299,36 +294,51 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
             apart |= up[n][j] > kLossless;
         }
     apart = __any_sync(0xffffffffu, apart);
-    // Where the page's values are 2^64 below the reference, its weights in units of u add nothing to the output, and fp32 may not hold them.
-    // They are taken in units of m, for the denominator, and are zero in the product.
+    // Where the page's values are 2^up below the reference, fp16 would lose every weight below 2^(up - 32) of the largest: there may be many,
+    // they count for the denominator, and for the output where the large values are zeros.  So u is lowered, and the sums are multiplied by
+    // as much, for which fp32 has room up to 2^100.  Where that does not suffice, the page's weights are for the denominator alone,
+    // in units of m, and add nothing to sums of that size.
+    bool far[NT][2];
     if (apart) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (up[n][j] > kFarApart) shift[n][j] = -w.m[n][j];
+            for (int j = 0; j < 2; ++j) {
+                float big = 0.f;
+#pragma unroll
+                for (int i = 0; i < Rows<D, NT>::kSteps; ++i) big = fmaxf(big, fmaxf(fabsf(w.o[i][n][j]), fabsf(w.o[i][n][j + 2])));
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const int room = min(100 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 120);
+                const int d = static_cast<int>(fmaxf(floorf(up[n][j]), 0.f));
+                far[n][j] = d > room;
+                const float lift = far[n][j] ? 1.f : exp2_int(d), by = far[n][j] ? 0.f : static_cast<float>(d);
+                w.u[n][j] -= by;
+                shift[n][j] = far[n][j] ? kHeadroom - w.m[n][j] : shift[n][j] + by;
+                up[n][j] = far[n][j] ? 0.f : up[n][j] - by;
+#pragma unroll
+                for (int i = 0; i < Rows<D, NT>::kSteps; ++i) {
+                    w.o[i][n][j] *= lift;
+                    w.o[i][n][j + 2] *= lift;
+                }
+            }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         float e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = ex2(fmaf(s[n][j], c[n][j & 1], shift[n][j & 1]));
+        // The denominator sums the weights as they are rounded for the product, so that a rounding common to both cancels: a token that takes
+        // nearly all is then exact.
         uint32_t lo = pack_half2(e[0], e[1]), hi = pack_half2(e[2], e[3]);
         const float2 a = unpack_half2(lo), b = unpack_half2(hi);
-        float sum[2] = {a.x + b.x, a.y + b.y};
+        w.l[n][0] = fmaf(a.x + b.x, ex2(up[n][0] - kHeadroom), w.l[n][0]);
+        w.l[n][1] = fmaf(a.y + b.y, ex2(up[n][1] - kHeadroom), w.l[n][1]);
         if (apart) {
-            sum[0] = counted(e[0], a.x) + counted(e[2], b.x);
-            sum[1] = counted(e[1], a.y) + counted(e[3], b.y);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (up[n][j] > kFarApart) {
-                    up[n][j] = kHeadroom;
-                    lo &= j ? 0xffffu : 0xffff0000u;
-                    hi &= j ? 0xffffu : 0xffff0000u;
-                }
+            const uint32_t keep = (far[n][0] ? 0u : 0xffffu) | (far[n][1] ? 0u : 0xffff0000u);
+            lo &= keep;
+            hi &= keep;
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) w.l[n][j] = fmaf(sum[j], ex2(up[n][j] - kHeadroom), w.l[n][j]);
         weights[n][0] = movmatrix_trans(lo);        // tokens 2t, 2t + 1 of column g
         weights[n][1] = movmatrix_trans(hi);
     }

@@ -25,8 +25,10 @@
 // from scores to weights to products and back (one group of eight products by itself 960 to 1120 cycles, 512 of them at work).
 // One tile a CTA with two buffers for scores: 580 us, as the codes are then converted for half as many rows.
 //
-// The pages' scales enter with the weights, as two numbers for each 16 columns of the scores: weight = 2^(s c_page + shift_page), so that
-// fp16 weights use their range whatever the scales are (page_weights in tq_attend8.cu has the same two references m and u).
+// K's scales enter with the weights, for each 16 columns of the scores: weight = 2^(s c_page + shift_page).  V's enter with the values where they are converted, as far as
+// fp16 holds those exactly: 22 powers of two below the largest scale seen so far.  What goes beyond enters with the weights, which
+// then use their range whatever the scales are (page_weights in tq_attend8.cu has the same two references m and u); pages 2^(22 + x) below
+// the largest lose weights below 2^(x - 32) of the largest, in the product, not in the denominator.
 // A NaN in V counts as zero in the product; its dim and token are noted, and rows that see the token become NaN in that dim at the end.
 //
 // All waits are bounded; one that gives up sets TQ_STATUS_TIMEOUT, every role leaves its loop, copies and products that are under way are waited
@@ -46,10 +48,13 @@ constexpr int kTilePages = kTile / kPageTokens;
 constexpr int kPlans = 8;
 constexpr int kRankedSeqs = 128;                // sequences that a CTA sorts by length
 
-// The scales of a tile's pages: of K as it is, of V as the power of two.
+// The scales of a tile's pages: of K as it is; of V a power of two in two parts, 2^v_exp for the weights and v_factor, fp16 bits, for the values.
 struct alignas(16) StepPlan {
     float k_scale[kTilePages], v_exp[kTilePages];
+    uint16_t v_factor[kTilePages];
 };
+// Codes are at most 2^8.8 and multiples of 2^-9: times 2^7 to 2^-15 fp16 holds them exactly.
+constexpr int kMostLift = 7, kLeastLift = -15;
 
 template <int D>
 struct PromptSmem {
@@ -151,13 +156,18 @@ struct PromptJob {
 };
 
 // 16 codes as fp16 into two 16-byte pieces.
-__device__ __forceinline__ void convert16(uint4 codes, uint32_t at, uint32_t step) {
+template <bool SCALED>
+__device__ __forceinline__ void convert16(uint4 codes, uint32_t at, uint32_t step, uint32_t factor) {
     const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
     uint32_t h[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
         h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
+        if (SCALED) {
+            asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[2 * i]) : "r"(factor));
+            asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[2 * i + 1]) : "r"(factor));
+        }
     }
     sts16(at, h[0], h[1], h[2], h[3]);
     sts16(at + step, h[4], h[5], h[6], h[7]);
@@ -186,6 +196,7 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         return page < pages ? __ldg(table + page / p.pages_per_block) : 0;
     };
     int block = ask_block(job.token_a), step = 0, keys = 0, values = 0;     // copies of tiles that were issued
+    int largest = kMinExponent - kMostLift;                                 // scale of V so far
     for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
         const int page = token0 / kPageTokens + mine, count = min(pages - token0 / kPageTokens, kTilePages);
         const bool here = mine < count;
@@ -196,6 +207,9 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         const uint8_t* at = here ? page_address<D>(p, page, block, job.kvh) : nullptr;
         block = ask_block(token0 + kTile);
         const float2 scales = here ? __ldg(reinterpret_cast<const float2*>(at + cache8_scale_off(D))) : make_float2(0.f, 0.f);
+        const int ev = static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127;
+        largest = max(largest, __reduce_max_sync(0xffffffffu, here ? ev : kMinExponent - kMostLift));
+        const int lift = here ? max(ev - largest + kMostLift, kLeastLift) : 0;
         // Pages that are not there keep the codes of another tile: their columns are masked, and finite values times zero are zero.
         const uint32_t turn = (step & 1) ^ 1;
         if (!waited(bars + kbRawKEmpty, turn, flags)) break;
@@ -208,7 +222,8 @@ __device__ void prompt_plan(const Attend8Params& p, const PromptJob& job, int se
         StepPlan& plan = plans[slot];
         if (lane < kTilePages) {
             plan.k_scale[mine] = scales.x;
-            plan.v_exp[mine] = here ? static_cast<float>(static_cast<int>(__float_as_uint(scales.y) >> 23 & 0xffu) - 127) : 0.f;
+            plan.v_exp[mine] = static_cast<float>(here ? ev - lift : largest - kMostLift);
+            plan.v_factor[mine] = static_cast<uint16_t>(lift == kLeastLift ? 0x200 : (lift + 15) << 10);
         }
         __syncwarp();
         if (lane == 0) {
@@ -240,6 +255,7 @@ __device__ void prompt_convert(const PromptJob& job, uint8_t* smem, uint64_t* ba
     const int tok = lane & 15, half = lane >> 4;
     const uint32_t base = smem_u32(smem), operand = base + (VALUES ? Smem::kV : Smem::kK), raw = base + (VALUES ? Smem::kRawV : Smem::kRawK);
     int* first_nan = reinterpret_cast<int*>(smem + Smem::kNan);
+    const StepPlan* plans = reinterpret_cast<const StepPlan*>(smem + Smem::kPlan);      // written before the copy of the values is asked for
     int step = 0;
     for (int token0 = job.token_a; token0 < job.token_b; token0 += kTile, ++step) {
         const int s = step & 1;
@@ -248,6 +264,7 @@ __device__ void prompt_convert(const PromptJob& job, uint8_t* smem, uint64_t* ba
         for (int i = 0; i < kPages; ++i) {
             const int token = (first + i) * kPageTokens + tok;
             const uint32_t to = operand + s * Smem::kOperand + (VALUES ? (token >> 3) * (D * 16) + (token & 7) * 16 : token * 16);
+            const uint32_t factor = VALUES ? plans[step % kPlans].v_factor[first + i] * 0x10001u : 0u;
             uint4 x[kLoads];
             uint32_t nan = 0;                                               // bit 7 of a byte: a code is 0x7f or 0xff
 #pragma unroll
@@ -257,7 +274,7 @@ __device__ void prompt_convert(const PromptJob& job, uint8_t* smem, uint64_t* ba
                 if (VALUES)
                     nan |= ((x[j].x & 0x7f7f7f7fu) + 0x01010101u) | ((x[j].y & 0x7f7f7f7fu) + 0x01010101u) |
                            ((x[j].z & 0x7f7f7f7fu) + 0x01010101u) | ((x[j].w & 0x7f7f7f7fu) + 0x01010101u);
-                convert16(x[j], to + ((2 * j + half) ^ (tok & (2 * kLoads - 1))) * 2 * kColumn, kColumn);
+                convert16<VALUES>(x[j], to + ((2 * j + half) ^ (tok & (2 * kLoads - 1))) * 2 * kColumn, kColumn, factor);
             }
             if (VALUES && (nan & 0x80808080u)) {
                 // rare: this lane's pieces once more, from where they were put
@@ -368,6 +385,12 @@ __device__ void prompt_multiply(const PromptJob& job, uint8_t* smem, uint64_t* b
     wait(kbDrained, 0);
 }
 
+constexpr float kFarApart = 60.f;           // values so many powers of two below the reference: fp32 may not hold the weights in its units
+
+// What a weight counts for in the denominator where the values lie further below the reference than the product's fp16 goes: as it was rounded, or, where
+// fp16 has no full precision (2^-14), as it is.
+__device__ __forceinline__ float counted(float weight, float rounded) { return weight < 6.103515625e-5f ? weight : rounded; }
+
 constexpr float kTiny = 1e-38f;             // factors of scores are never zero: times -inf that would be NaN
 
 // Columns from `visible` on see nothing.
@@ -451,7 +474,7 @@ __device__ void prompt_softmax(const Attend8Params& p, const PromptJob& job, int
                         z = ex2(z);
                         w[8 * g + i] = pack_half2(y, z);
                         if (!BF16) {
-                            // as they are rounded for the product (counted()); an output in bf16 does not show the difference
+                            // as they are rounded for the product (page_weights); an output in bf16 does not show the difference
                             const float2 v = unpack_half2(w[8 * g + i]);
                             y = decltype(cut)::value ? counted(y, v.x) : v.x;
                             z = decltype(cut)::value ? counted(z, v.y) : v.y;

@@ -26,7 +26,7 @@ __host__ __device__ __forceinline__ int exponent_of_scale_bits(uint32_t scale_bi
     return e < kMinExponent || e > kMaxExponent ? kMinExponent : e;
 }
 
-__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }   // |e| <= 126
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }   // |e| <= 126; -127 makes zero
 
 // two floats -> two e4m3 codes, lo in bits 0..7; nearest even, saturating (infinities too), NaN stays one
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {

@@ -283,23 +283,17 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
                 w.u[n][j] = u;
             }
     }
-    float up[NT][2], shift[NT][2];
     bool apart = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            up[n][j] = w.u[n][j] - ev - w.m[n][j];
-            shift[n][j] = ev + kHeadroom - w.u[n][j];
-            apart |= up[n][j] > kLossless;
-        }
-    apart = __any_sync(0xffffffffu, apart);
+        for (int j = 0; j < 2; ++j) apart |= w.u[n][j] - ev - w.m[n][j] > kLossless;
     // Where the page's values are 2^up below the reference, fp16 would lose every weight below 2^(up - 32) of the largest: there may be many,
     // they count for the denominator, and for the output where the large values are zeros.  So u is lowered, and the sums are multiplied by
     // as much, for which fp32 has room up to 2^100.  Where that does not suffice, the page's weights are for the denominator alone,
     // in units of m, and add nothing to sums of that size.
-    bool far[NT][2];
-    if (apart) {
+    uint32_t far = 0;                   // bit 2 n + j
+    if (__any_sync(0xffffffffu, apart)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -310,12 +304,13 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
                 const int room = min(100 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 120);
-                const int d = static_cast<int>(fmaxf(floorf(up[n][j]), 0.f));
-                far[n][j] = d > room;
-                const float lift = far[n][j] ? 1.f : exp2_int(d), by = far[n][j] ? 0.f : static_cast<float>(d);
-                w.u[n][j] -= by;
-                shift[n][j] = far[n][j] ? kHeadroom - w.m[n][j] : shift[n][j] + by;
-                up[n][j] = far[n][j] ? 0.f : up[n][j] - by;
+                int d = static_cast<int>(fmaxf(floorf(w.u[n][j] - ev - w.m[n][j]), 0.f));
+                if (d > room) {
+                    far |= 1u << (2 * n + j);
+                    d = 0;
+                }
+                const float lift = exp2_int(d);
+                w.u[n][j] -= static_cast<float>(d);
 #pragma unroll
                 for (int i = 0; i < Rows<D, NT>::kSteps; ++i) {
                     w.o[i][n][j] *= lift;
@@ -325,17 +320,26 @@ __device__ __forceinline__ void page_weights(Rows<D, NT>& w, float (&s)[NT][4], 
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        float e[4];
+        float shift[2], unit[2], e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = ex2(fmaf(s[n][j], c[n][j & 1], shift[n][j & 1]));
+        for (int j = 0; j < 2; ++j) {
+            shift[j] = ev + kHeadroom - w.u[n][j];
+            unit[j] = -shift[j] - w.m[n][j];
+            if (far >> (2 * n + j) & 1) {
+                shift[j] = kHeadroom - w.m[n][j];
+                unit[j] = -kHeadroom;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = ex2(fmaf(s[n][j], c[n][j & 1], shift[j & 1]));
         // The denominator sums the weights as they are rounded for the product, so that a rounding common to both cancels: a token that takes
         // nearly all is then exact.
         uint32_t lo = pack_half2(e[0], e[1]), hi = pack_half2(e[2], e[3]);
         const float2 a = unpack_half2(lo), b = unpack_half2(hi);
-        w.l[n][0] = fmaf(a.x + b.x, ex2(up[n][0] - kHeadroom), w.l[n][0]);
-        w.l[n][1] = fmaf(a.y + b.y, ex2(up[n][1] - kHeadroom), w.l[n][1]);
-        if (apart) {
-            const uint32_t keep = (far[n][0] ? 0u : 0xffffu) | (far[n][1] ? 0u : 0xffff0000u);
+        w.l[n][0] = fmaf(a.x + b.x, ex2(unit[0]), w.l[n][0]);
+        w.l[n][1] = fmaf(a.y + b.y, ex2(unit[1]), w.l[n][1]);
+        if (far) {
+            const uint32_t keep = (far >> (2 * n) & 1 ? 0u : 0xffffu) | (far >> (2 * n + 1) & 1 ? 0u : 0xffff0000u);
             lo &= keep;
             hi &= keep;
         }

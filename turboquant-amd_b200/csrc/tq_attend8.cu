@@ -6,7 +6,7 @@
 //   out = sum_k 2^(s_k - m) vscale(page of k) V_k / sum_k 2^(s_k - m)      (s in units of log2)
 //
 // Bound: HBM, the 2 D + 2 bytes of a cached token and head.  8 query rows take D / 8 products (m16n8k16) a page of 16 tokens; with D = 128 the persistent
-// kernel issues 348 warp instructions a page in all, at half of the issue slots.
+// kernel issues 359 warp instructions a page in all, at half of the issue slots.
 #include "tq_cache8.cuh"
 
 namespace tq {
@@ -681,7 +681,7 @@ constexpr int64_t kStreamPages = 32768;
 Attend8Plan attend8_plan(int64_t num_rows, int64_t seqs, int kv_heads, int group, int max_queries, int max_pages) {
     Attend8Plan a = {};
     const int64_t rows = static_cast<int64_t>(group) * max_queries;
-    // (64 x 8192 tokens, 64 / 8 heads: 32 rows are 427 us in tiles of 16 rows, 64 rows 667 in one tile of 256, both fp16.)
+    // (64 x 8192 tokens, 64 / 8 heads: 32 rows are 428 to 440 us in tiles of 16 rows, 64 rows 667 in one tile of 256, both fp16.)
     if (rows > 32) {
         a.kind = Attend8Kind::kPrompt;
         a.tiles = (rows + 2 * kTile - 1) / (2 * kTile) * seqs;
@@ -689,7 +689,7 @@ Attend8Plan attend8_plan(int64_t num_rows, int64_t seqs, int kv_heads, int group
         if (full + seqs < a.tiles) a.tiles = full + seqs;
         int64_t items = a.tiles;
         // Decodes next to a chunk: a tile of 256 rows with 4 or 8 in use costs what a full one does.  (32 / 8 heads, 64 decodes over 8192 tokens and a
-        // chunk of 2048: 605 us, 1222 by one kernel; 200 over 1024 and two of 1024: 206, 639; 8 over 4096 and four of 512: 271, 288.)
+        // chunk of 2048: 606 us, 1222 by one kernel; 200 over 1024 and two of 1024: 207, 639; 8 over 4096 and four of 512: 275, 288.)
         if (group <= 16 && num_rows < seqs * max_queries && seqs * kv_heads * max_pages >= kStreamPages) {
             a.small_rows = 16;
             a.nt = group <= 8 ? 1 : 2;

@@ -20,8 +20,8 @@
 // So loops stay loops here, the codes go through shared memory instead of registers, and steps without hidden columns have a
 // loop without masks (482 us with one for both).
 //
-// 32 / 8 heads of 128, bf16: 4 chunks of 700 to 1024 tokens over 1000 to 7168 452 us (658 TFLOP/s; fp16 481), one of 2048 over 16384 730-740
-// (790-800), one of 4096 over nothing 210 (655).  A step of two tiles takes 2.6 to 2.9 us, 1.1 of them products: what is left is the chain
+// 32 / 8 heads of 128, bf16: 4 chunks of 700 to 1024 tokens over 1000 to 7168 453 us (658 TFLOP/s; fp16 492), one of 2048 over 16384 730-740
+// (790-800), one of 4096 over nothing 213 (646).  A step of two tiles takes 2.6 to 2.9 us, 1.1 of them products: what is left is the chain
 // from scores to weights to products and back (one group of eight products by itself 960 to 1120 cycles, 512 of them at work).
 // One tile a CTA with two buffers for scores: 580 us, as the codes are then converted for half as many rows.
 //

@@ -8,7 +8,7 @@
 // tokens, four pieces) and of values (four tokens two apart, two pieces) touch all banks once.
 //
 // 64 / 8 heads of 128, fp16, 64 sequences of 8192 tokens: 185 us = 5.8 TB/s, 0.89 of a copy; 64 uneven ones of bf16 74 us, 0.73.  What is missing: 4 us to the
-// first page, CTAs that end within 6 % of one another, joins and merge (7 us).  348 warp instructions a page at half of the issue slots.
+// first page, CTAs that end within 6 % of one another, joins and merge (7 us).  359 warp instructions a page at half of the issue slots.
 //
 // Whole items are written from registers.  Parts are joined in shared memory by the CTA, and what crosses CTAs goes to the workspace, at
 // most two parts a CTA, for a second kernel.

@@ -94,7 +94,7 @@ def _frequencies(rotary_dim: int, max_position: int, base: float, scaling: Optio
     freq = freq * (1 - stretch) + freq / factor * stretch
     if "attention_factor" in spec:
         return freq, float(spec["attention_factor"])
-    if spec.get("mscale") and spec.get("mscale_all_dim"):
+    if spec.get("mscale") and spec.get("mscale_all_dim"):             # as configurations define it: one without the other changes nothing
         return freq, size_of(float(spec["mscale"])) / size_of(float(spec["mscale_all_dim"]))
     return freq, size_of(1.0)
 
